@@ -45,6 +45,7 @@ extern "C" {
 #define B2_F16 1
 #define B2_BF16 2
 #define B2_I64 3
+#define B2_I32 4 /* positions and slots only */
 
 /* GEMM epilogue activations (reference op table: triton_msl/codegen/_lowerer_templates.py:1733-1748) */
 #define B2_ACT_NONE 0
@@ -253,15 +254,109 @@ int b2_row_reduce_noalloc(int op, const void* x, void* out, int64_t rows, int64_
 int b2_reduce_axis(int op, const void* x, void* out, int64_t outer, int64_t R, int64_t inner,
                    int dtype, void* workspace, size_t ws_bytes, void* stream);
 
+/*
+ * ---- Decoder serving ----
+ * The operators around a decoder layer's attention: q/k norm with rotary
+ * positions, a paged key/value cache in 4 bits, attention over it, and causal
+ * attention over packed prompts. No counterparts in the reference.
+ * Index operands (positions, slots, page tables, lengths, offsets) live on the
+ * device; one that points outside what it indexes is never followed: it sets
+ * B2_STATUS_BAD_INDEX and yields what each entry says.
+ */
+
+/*
+ * q_out, k_out = rotate(norm(q)), rotate(norm(k)) over q[T, Hq, D], k[T, Hk, D].
+ * norm(x) = x * rsqrt(mean_d(x^2) + eps) * weight per token and head, or x where
+ * the weight [D] is NULL. rotate: with (c, s) = (table[p][i], table[p][R/2 + i]),
+ * p the token's position, each of the R/2 pairs (a, b) becomes (a*c - b*s,
+ * b*c + a*s); the pairs are channels (i, i + R/2), or (2i, 2i + 1) when
+ * interleaved; channels R..D-1 are not rotated. table is fp32 [P, R]; positions
+ * [T] of pos_dtype B2_I32 or B2_I64; a position outside [0, P) makes the token's
+ * rotated channels NaN. strides[8] = {q.t, q.h, k.t, k.h, q_out.t, q_out.h,
+ * k_out.t, k_out.h} in elements, unit channel stride; weights have `dtype`.
+ * q_out may be q and k_out may be k (same strides). D and R even, D <= 512.
+ */
+int b2_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, const void* q_weight,
+                    const void* k_weight, const float* table, const void* positions, int pos_dtype,
+                    int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t R, int64_t P,
+                    const int64_t strides[8], float eps, int interleaved, int dtype, void* stream);
+
+/*
+ * The 4-bit paged cache. cache[5] = {pages, H, page_size, D, group}; D is 64 or
+ * 128, group 64 or D. Four contiguous arrays starting on 16-byte boundaries:
+ *   k_codes, v_codes: uint8 [pages, H, page_size, D/2], 32-bit words of 8
+ *     channels (the first in the lowest bits), the word of channels 64g+8i.. at
+ *     word i*(D/64)+g of the row;
+ *   k_scales, v_scales: bf16 [pages, H, page_size, D/group, 2] = (scale, low).
+ * A code c stands for c*scale + low, with low = min of the group rounded down to
+ * bf16, scale = (max - low)/15 rounded up to bf16 and c = rint((x - low)/scale).
+ * A group that holds a NaN or an infinity reads back as NaN.
+ * Slot s is token s % page_size of page s / page_size.
+ *
+ * b2_kv_cache_write: quantises k[T, H, D] and v[T, H, D] into slots[T] (B2_I32 or
+ * B2_I64). A negative slot is padding and is not written; one past the cache is
+ * not written either and sets the status. The slots of one call must differ.
+ * b2_kv_cache_read: k[t], v[t] = the values of slots[t], rounded to `dtype`;
+ * zeros for a negative slot, NaN for one past the cache.
+ * strides[4] = {k.t, k.h, v.t, v.h} in elements, unit channel stride.
+ */
+int b2_kv_cache_write(const void* k, const void* v, void* k_codes, void* k_scales, void* v_codes,
+                      void* v_scales, const void* slots, int slots_dtype, int64_t T,
+                      const int64_t cache[5], const int64_t strides[4], int dtype, void* stream);
+int b2_kv_cache_read(void* k, void* v, const void* k_codes, const void* k_scales, const void* v_codes,
+                     const void* v_scales, const void* slots, int slots_dtype, int64_t T,
+                     const int64_t cache[5], const int64_t strides[4], int dtype, void* stream);
+
+/*
+ * Attention of the newest N tokens of each of B sequences over the 4-bit cache:
+ * o[b, n, h] = softmax_j(sm_scale * q[b, n, h] . k_j) v_j over the tokens
+ * j < lengths[b] - N + 1 + n of the sequence (its own position and all before),
+ * which lie in pages page_table[b][j / page_size]; query head h reads cache head
+ * h / (Hq / H). lengths[b] (int32) counts the N new tokens, already written. A
+ * row without a key gives zeros; a page outside the cache, or a length that is
+ * negative or longer than max_pages * page_size, makes the sequence's rows NaN.
+ * What the cache holds past a sequence's length cannot reach the result.
+ * page_table is int32 [B, max_pages] with row stride table_stride; page_size a
+ * multiple of 16; strides[6] = {q.b, q.n, q.h, o.b, o.n, o.h}, unit channel stride.
+ * workspace: b2_query_workspace(4, B, N*Hq/H, H, D) bytes, 16-byte aligned.
+ */
+int b2_kv_cache_attn(const void* q, void* o, const void* k_codes, const void* k_scales,
+                     const void* v_codes, const void* v_scales, const int32_t* page_table,
+                     const int32_t* lengths, int64_t B, int64_t N, int64_t Hq, int64_t max_pages,
+                     int64_t table_stride, const int64_t cache[5], const int64_t strides[6],
+                     float sm_scale, int dtype, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Attention over packed sequences: tokens cu_q[b] .. cu_q[b+1] of q[Tq, Hq, D]
+ * attend tokens cu_k[b] .. cu_k[b+1] of k, v[Tk, Hk, D] (int32 offsets [B+1]).
+ * Causal: query i of a sequence keeps the keys j <= i + (Lk - Lq). Query head h
+ * reads key head h / (Hq / Hk). A query without a key, and a token outside every
+ * sequence, gives zeros. Other sequences' keys and masked keys cannot reach a
+ * result, whatever they hold. Offsets must ascend within [0, T]; others are
+ * clamped and set the status. strides[12] = {t, h, d} of q, k, v, o in elements.
+ * fp16/bf16 with D a multiple of 8, unit channel stride, strides that are
+ * multiples of 8 and 16-byte aligned pointers run on the tensor cores given the
+ * workspace b2_query_workspace(5, B, Tq, Hq/Hk) reports (16-byte aligned); the
+ * rest, and sm_scale <= 0, on the CUDA cores. D <= 128.
+ */
+int b2_fa_packed(const void* q, const void* k, const void* v, void* o, const int32_t* cu_q,
+                 const int32_t* cu_k, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk,
+                 int64_t D, const int64_t strides[12], float sm_scale, int causal, int dtype,
+                 void* workspace, size_t ws_bytes, void* stream);
+
 /* Scratch bytes a call with these arguments needs (0 = none).
  * kind: 0 = b2_gemm (a0=M, a1=N, a2=K, a3=in_dtype),
  *       1 = b2_row_op (a0=op, a1=rows, a2=cols, a3=dtype),
  *       2 = b2_fa_fwd (always 0),
- *       3 = b2_reduce_axis (a0=outer, a1=R, a2=inner). */
+ *       3 = b2_reduce_axis (a0=outer, a1=R, a2=inner),
+ *       4 = b2_kv_cache_attn (a0=B, a1=N*Hq/H, a2=H, a3=D),
+ *       5 = b2_fa_packed (a0=B, a1=Tq, a2=Hq/Hk). */
 size_t b2_query_workspace(int kind, int64_t a0, int64_t a1, int64_t a2, int64_t a3);
 
-/* OR of the device status bits written by bounded waits on `device` since the
- * last clear (0 = no wait expired). Synchronises that device. clear != 0 resets it. */
+/* OR of the device status bits written by kernels on `device` since the last
+ * clear (0 = none). Returns B2_ETIMEOUT when a bounded wait expired, B2_EINVAL
+ * when only B2_STATUS_BAD_INDEX is set. Synchronises that device. clear != 0
+ * resets it. */
 int b2_device_status(int device, int clear, uint32_t* status_out);
 
 /* Device status bits (b2_device_status). */
@@ -269,6 +364,8 @@ int b2_device_status(int device, int clear, uint32_t* status_out);
 #define B2_STATUS_TIMEOUT_MMA 0x2u  /* a waiter gave up on a tensor-core commit */
 #define B2_STATUS_TIMEOUT_EPI 0x4u  /* a waiter gave up on the epilogue / softmax warps */
 #define B2_STATUS_TIMEOUT_SLOT 0x8u /* the TMA producer gave up waiting for a free stage */
+#define B2_STATUS_BAD_INDEX 0x10u   /* a position, slot, page or offset of a decoder-serving call
+                                       pointed outside what it indexes (nothing was accessed there) */
 
 /*
  * Failure-path test of the bounded device waits (no counterpart in the

@@ -18,8 +18,9 @@ PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("B2MSL_LIBRARY", PKG / "libb2msl.so"))
 
 B2_OK, B2_EINVAL, B2_EUNSUPPORTED, B2_ELAUNCH, B2_ETIMEOUT = 0, -1, -2, -3, -4
-B2_F32, B2_F16, B2_BF16, B2_I64 = 0, 1, 2, 3
+B2_F32, B2_F16, B2_BF16, B2_I64, B2_I32 = 0, 1, 2, 3, 4
 STATUS_TIMEOUT_TMA, STATUS_TIMEOUT_MMA, STATUS_TIMEOUT_EPI, STATUS_TIMEOUT_SLOT = 1, 2, 4, 8
+STATUS_BAD_INDEX = 16
 ACT = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "softmax": 5}
 # b2_gemm_epilogue op codes (B2_EPI_* in include/b2msl.h) and their constant counts
 EPI = {"add": (1, 1), "sub": (2, 1), "rsub": (3, 1), "mul": (4, 1), "div": (5, 1),
@@ -59,6 +60,18 @@ SIGNATURES = {
                               + [ctypes.c_int64] * 3 + [ctypes.c_int, ctypes.c_void_p]),
     "b2_test_stalled_gemm": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_int64] * 3
                              + [ctypes.c_uint64, ctypes.c_void_p]),
+    "b2_qk_norm_rope": (ctypes.c_int, [ctypes.c_void_p] * 8 + [ctypes.c_int] + [ctypes.c_int64] * 6
+                        + [_c_i64p, ctypes.c_float, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]),
+    "b2_kv_cache_write": (ctypes.c_int, [ctypes.c_void_p] * 7 + [ctypes.c_int, ctypes.c_int64, _c_i64p,
+                                                                 _c_i64p, ctypes.c_int, ctypes.c_void_p]),
+    "b2_kv_cache_read": (ctypes.c_int, [ctypes.c_void_p] * 7 + [ctypes.c_int, ctypes.c_int64, _c_i64p,
+                                                                _c_i64p, ctypes.c_int, ctypes.c_void_p]),
+    "b2_kv_cache_attn": (ctypes.c_int, [ctypes.c_void_p] * 8 + [ctypes.c_int64] * 5
+                         + [_c_i64p, _c_i64p, ctypes.c_float, ctypes.c_int, ctypes.c_void_p,
+                            ctypes.c_size_t, ctypes.c_void_p]),
+    "b2_fa_packed": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_int64] * 6
+                     + [_c_i64p, ctypes.c_float, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                        ctypes.c_size_t, ctypes.c_void_p]),
     "b2_query_workspace": (ctypes.c_size_t, [ctypes.c_int] + [ctypes.c_int64] * 4),
     "b2_device_status": (ctypes.c_int, [ctypes.c_int, ctypes.c_int,
                                         ctypes.POINTER(ctypes.c_uint32)]),
@@ -123,6 +136,6 @@ def last_kernel() -> str:
 def device_status(device: int, clear: bool = True) -> int:
     out = ctypes.c_uint32(0)
     st = lib().b2_device_status(int(device), 1 if clear else 0, ctypes.byref(out))
-    if st not in (B2_OK, B2_ETIMEOUT):
+    if st not in (B2_OK, B2_ETIMEOUT, B2_EINVAL):  # EINVAL: only STATUS_BAD_INDEX is set
         check("b2_device_status", st)
     return int(out.value)

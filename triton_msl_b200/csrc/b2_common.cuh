@@ -28,6 +28,7 @@ enum : uint32_t {
   DEV_TIMEOUT_MMA = 1u << 1,    // a waiter gave up on a tensor-core commit
   DEV_TIMEOUT_EPI = 1u << 2,    // an epilogue/softmax waiter gave up
   DEV_TIMEOUT_SLOT = 1u << 3,   // a producer gave up waiting for a free slot
+  DEV_BAD_INDEX = 1u << 4,      // an index operand pointed outside what it indexes
 };
 
 // Upper bound on any single spin inside a kernel. Every legitimate wait in
@@ -40,6 +41,7 @@ inline int dtype_size(int dt) {
     case B2_F16: return 2;
     case B2_BF16: return 2;
     case B2_I64: return 8;
+    case B2_I32: return 4;
     default: return 0;
   }
 }
@@ -50,6 +52,7 @@ inline const char* dtype_name(int dt) {
     case B2_F16: return "f16";
     case B2_BF16: return "bf16";
     case B2_I64: return "i64";
+    case B2_I32: return "i32";
     default: return "?";
   }
 }

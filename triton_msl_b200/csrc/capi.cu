@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "b2_common.cuh"
+#include "decoder.cuh"
 
 namespace b2 {
 
@@ -48,6 +49,7 @@ thread_local const char* t_kernel = "";
 constexpr int kMaxDev = 64;
 int g_cc_major[kMaxDev];
 std::once_flag g_cc_once[kMaxDev];
+}  // namespace
 
 bool device_is_sm100() {
   int dev = 0;
@@ -60,6 +62,9 @@ bool device_is_sm100() {
   return g_cc_major[dev] == 10;
 }
 
+void set_last_kernel(const char* name) { t_kernel = name; }
+
+namespace {
 int g_sm_count[kMaxDev];
 std::once_flag g_sm_once[kMaxDev];
 
@@ -367,6 +372,8 @@ size_t b2_query_workspace(int kind, int64_t a0, int64_t a1, int64_t a2, int64_t 
     case 1: return row_op_workspace((int)a0, a1, a2);
     case 2: return 0;
     case 3: return axis_reduce_workspace(a0, a1, a2);
+    case 4: return kv_cache_attn_workspace(a0, a1, a2, a3);
+    case 5: return fa_packed_workspace(a0, a1, a2);
     default: return 0;
   }
 }
@@ -410,6 +417,7 @@ int b2_device_status(int device, int clear, uint32_t* status_out) {
     s |= gemm_read_status(clear != 0);
     s |= pair_read_status(clear != 0);
     s |= fa_read_status(clear != 0);
+    s |= decoder_read_status(clear != 0);
     e = cudaGetLastError();
   }
   cudaSetDevice(prev);
@@ -418,7 +426,7 @@ int b2_device_status(int device, int clear, uint32_t* status_out) {
     return B2_ELAUNCH;
   }
   if (status_out) *status_out = s;
-  return s ? B2_ETIMEOUT : B2_OK;
+  return (s & ~(uint32_t)DEV_BAD_INDEX) ? B2_ETIMEOUT : s ? B2_EINVAL : B2_OK;
 }
 
 }  // extern "C"

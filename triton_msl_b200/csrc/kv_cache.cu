@@ -1,0 +1,266 @@
+// The paged key/value cache in 4 bits: quantising rows as they are written, and
+// reading rows back.
+//
+// A row is one token's D channels of one head. Each group of 64 or 128 channels
+// is held as codes c in 0..15 with a scale s and a lowest value lo in bf16:
+//   lo = min rounded down to bf16, s = (max - lo) * (1/15) rounded up to bf16,
+//   c = clamp(rint((x - lo) * (1/s)), 0, 15) in fp32, read back as c*s + lo.
+// Rounding lo down and s up keeps the whole range inside codes 0..15, so no
+// value is clipped by more than half a step; bf16 because it has fp32's range
+// (an outlier cannot overflow it) at 4 bytes a group, and its 8 bits widen the
+// step by at most 1/64. A group with a NaN or an infinity reads back as NaN.
+//
+// Layout: codes [pages, H, page, D/2]; the row's 32-bit words hold 8 channels,
+// the first in the lowest bits; the word with channels 64g+8i.. is stored at
+// word i*(D/64)+g, so that the 16 bytes which an attention lane loads hold words
+// of every 64-channel group and each tensor-core step stays inside one group
+// (kv_attn.cu). Scales [pages, H, page, D/group, 2].
+//
+// Bound: HBM. One thread owns one word of keys and the same word of values; a
+// group's extremes take 3 or 4 shuffles.
+#include "b2_common.cuh"
+#include "decoder.cuh"
+
+namespace b2 {
+namespace {
+
+__device__ uint32_t g_kv_cache_status;
+
+constexpr int kCacheThreads = 256;
+
+// max that keeps NaN (a group with a NaN has to be seen)
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// x rounded toward -inf to a bf16 value (finite x)
+__device__ __forceinline__ float bf16_down(float x) {
+  const int bits = __float_as_int(x), cut = bits & 0xffff0000;
+  return __int_as_float(bits < 0 && cut != bits ? cut + 0x10000 : cut);
+}
+// x >= 0 rounded up to a bf16 value
+__device__ __forceinline__ float bf16_up(float x) {
+  return __int_as_float((__float_as_int(x) + 0xffff) & 0xffff0000);
+}
+
+struct RowsArgs {
+  uint32_t *k_codes, *k_scales, *v_codes, *v_scales;  // words of 8 codes; (scale, lo) pairs
+  void *k, *v;
+  const void* slots;
+  long long kt, kh, vt, vh;
+  unsigned rows, H, page_size, capacity;
+  int slots64;
+};
+
+// 8 values of one row
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  if constexpr (VEC) {
+    uint4 r[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
+    const T* e = reinterpret_cast<const T*>(r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(p[i]);
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  if constexpr (VEC) {
+    uint4 r[sizeof(T) / 2];
+    T* e = reinterpret_cast<T*>(r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(f[i]);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = from_f32<T>(f[i]);
+  }
+}
+
+// The code word of 8 values and the group's (scale, lo) as two packed bf16.
+template <int LANES>
+__device__ __forceinline__ uint32_t quantise(const float (&x)[8], uint32_t& meta) {
+  float hi = x[0], lo = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    hi = max_nan(hi, x[i]);
+    lo = fminf(lo, x[i]);
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+  }
+  const float low = bf16_down(lo);
+  const float step = (hi - low) * (1.0f / 15.0f);
+  const float scale = bf16_up(step);
+  if (!(step < INFINITY) || !(scale < INFINITY)) {  // a NaN or an infinity in the group
+    meta = 0x7fff7fffu;
+    return 0u;
+  }
+  meta = (__float_as_uint(scale) >> 16) | (__float_as_uint(low) & 0xffff0000u);
+  // below 2^-126 the reciprocal may overflow; the group reads back as lo then
+  const float inv = scale >= 1.17549435e-38f ? 1.0f / scale : 0.0f;
+  // adding 1.5 * 2^23 rounds to the nearest integer (ties to even) and leaves it
+  // in the low bits; the constant's own bits add up to the number subtracted.
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = fminf((x[i] - low) * inv, 15.0f) + 12582912.0f;
+    word += (__float_as_uint(t) & 15u) << (4 * i);
+  }
+  return word;
+}
+
+template <int D>
+__device__ __forceinline__ int stored_word(int lane) {
+  return (lane & 7) * (D / 64) + (lane >> 3);
+}
+
+template <typename T, int D, int GROUP, bool VEC>
+__global__ void __launch_bounds__(kCacheThreads) kv_write_kernel(const __grid_constant__ RowsArgs a) {
+  constexpr int LPR = D / 8;
+  const unsigned tid = blockIdx.x * kCacheThreads + threadIdx.x;
+  const unsigned row = tid / LPR;
+  const int lane = tid % LPR;
+  // threads past the last row repeat it without storing: the shuffles need them
+  const unsigned r = row < a.rows ? row : a.rows - 1;
+  const unsigned token = r / a.H, head = r - token * a.H;
+  float k[8], v[8];
+  load8<T, VEC>(static_cast<const T*>(a.k) + (long long)token * a.kt + (long long)head * a.kh + lane * 8, k);
+  load8<T, VEC>(static_cast<const T*>(a.v) + (long long)token * a.vt + (long long)head * a.vh + lane * 8, v);
+  const long long slot = a.slots64 ? static_cast<const long long*>(a.slots)[token]
+                                   : static_cast<const int*>(a.slots)[token];
+  uint32_t mk, mv;
+  const uint32_t wk = quantise<GROUP / 8>(k, mk), wv = quantise<GROUP / 8>(v, mv);
+  if (row >= a.rows || slot < 0) return;
+  if (slot >= (long long)a.capacity) {
+    if (lane == 0) atomicOr(&g_kv_cache_status, DEV_BAD_INDEX);
+    return;
+  }
+  const unsigned page = (unsigned)slot / a.page_size, place = (unsigned)slot - page * a.page_size;
+  const size_t at = ((size_t)page * a.H + head) * a.page_size + place;
+  a.k_codes[at * LPR + stored_word<D>(lane)] = wk;
+  a.v_codes[at * LPR + stored_word<D>(lane)] = wv;
+  if (lane % (GROUP / 8) == 0) {
+    a.k_scales[at * (D / GROUP) + lane / (GROUP / 8)] = mk;
+    a.v_scales[at * (D / GROUP) + lane / (GROUP / 8)] = mv;
+  }
+}
+
+__device__ __forceinline__ void values8(uint32_t word, uint32_t meta, float (&f)[8]) {
+  const float s = __uint_as_float(meta << 16), lo = __uint_as_float(meta & 0xffff0000u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // 2^23 + c minus 2^23 is the code as a float
+    const float c = __uint_as_float(0x4b000000u | ((word >> (4 * i)) & 15u)) - 8388608.0f;
+    f[i] = fmaf(c, s, lo);
+  }
+}
+
+template <typename T, int D, int GROUP, bool VEC>
+__global__ void __launch_bounds__(kCacheThreads) kv_read_kernel(const __grid_constant__ RowsArgs a) {
+  constexpr int LPR = D / 8;
+  const unsigned tid = blockIdx.x * kCacheThreads + threadIdx.x;
+  const unsigned row = tid / LPR;
+  const int lane = tid % LPR;
+  if (row >= a.rows) return;
+  const unsigned token = row / a.H, head = row - token * a.H;
+  const long long slot = a.slots64 ? static_cast<const long long*>(a.slots)[token]
+                                   : static_cast<const int*>(a.slots)[token];
+  float k[8], v[8];
+  if (slot >= 0 && slot < (long long)a.capacity) {
+    const unsigned page = (unsigned)slot / a.page_size, place = (unsigned)slot - page * a.page_size;
+    const size_t at = ((size_t)page * a.H + head) * a.page_size + place;
+    const uint32_t wk = a.k_codes[at * LPR + stored_word<D>(lane)];
+    const uint32_t wv = a.v_codes[at * LPR + stored_word<D>(lane)];
+    const uint32_t mk = a.k_scales[at * (D / GROUP) + lane / (GROUP / 8)];
+    const uint32_t mv = a.v_scales[at * (D / GROUP) + lane / (GROUP / 8)];
+    values8(wk, mk, k);
+    values8(wv, mv, v);
+  } else {
+    // a negative slot is padding and reads as zero; one past the cache as NaN
+    const float fill = slot < 0 ? 0.f : __int_as_float(0x7fffffff);
+    if (slot >= 0 && lane == 0) atomicOr(&g_kv_cache_status, DEV_BAD_INDEX);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] = v[i] = fill;
+  }
+  store8<T, VEC>(static_cast<T*>(a.k) + (long long)token * a.kt + (long long)head * a.kh + lane * 8, k);
+  store8<T, VEC>(static_cast<T*>(a.v) + (long long)token * a.vt + (long long)head * a.vh + lane * 8, v);
+}
+
+template <bool WRITE, typename T, int D, int GROUP>
+int launch(const RowsArgs& a, bool vec, cudaStream_t st) {
+  const unsigned long long threads = (unsigned long long)a.rows * (D / 8);
+  const unsigned grid = (unsigned)((threads + kCacheThreads - 1) / kCacheThreads);
+  if constexpr (WRITE) {
+    if (vec) kv_write_kernel<T, D, GROUP, true><<<grid, kCacheThreads, 0, st>>>(a);
+    else kv_write_kernel<T, D, GROUP, false><<<grid, kCacheThreads, 0, st>>>(a);
+  } else {
+    if (vec) kv_read_kernel<T, D, GROUP, true><<<grid, kCacheThreads, 0, st>>>(a);
+    else kv_read_kernel<T, D, GROUP, false><<<grid, kCacheThreads, 0, st>>>(a);
+  }
+  B2_CHECK_LAUNCH();
+  return B2_OK;
+}
+
+template <bool WRITE, typename T>
+int launch_typed(const RowsArgs& a, const CacheShape& s, bool vec, cudaStream_t st) {
+  if (s.D == 64) return launch<WRITE, T, 64, 64>(a, vec, st);
+  if (s.group == 64) return launch<WRITE, T, 128, 64>(a, vec, st);
+  return launch<WRITE, T, 128, 128>(a, vec, st);
+}
+
+template <bool WRITE>
+int rows_launch(const CacheRowsCall& c, cudaStream_t st) {
+  const CacheShape& s = c.shape;
+  RowsArgs a = {};
+  a.k_codes = static_cast<uint32_t*>(c.k_codes);
+  a.k_scales = static_cast<uint32_t*>(c.k_scales);
+  a.v_codes = static_cast<uint32_t*>(c.v_codes);
+  a.v_scales = static_cast<uint32_t*>(c.v_scales);
+  a.k = c.k;
+  a.v = c.v;
+  a.slots = c.slots;
+  a.slots64 = c.slots64;
+  a.kt = c.strides[0];
+  a.kh = c.strides[1];
+  a.vt = c.strides[2];
+  a.vh = c.strides[3];
+  a.rows = (unsigned)(c.T * s.H);
+  a.H = (unsigned)s.H;
+  a.page_size = (unsigned)s.page_size;
+  a.capacity = (unsigned)(s.pages * s.page_size);
+  const long long per = 16 / dtype_size(c.dtype);
+  const bool vec = ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15) == 0 &&
+                   a.kt % per == 0 && a.kh % per == 0 && a.vt % per == 0 && a.vh % per == 0;
+  switch (c.dtype) {
+    case B2_F32: return launch_typed<WRITE, float>(a, s, vec, st);
+    case B2_F16: return launch_typed<WRITE, __half>(a, s, vec, st);
+    default: return launch_typed<WRITE, __nv_bfloat16>(a, s, vec, st);
+  }
+}
+
+}  // namespace
+
+int kv_cache_write_launch(const CacheRowsCall& c, cudaStream_t st) { return rows_launch<true>(c, st); }
+int kv_cache_read_launch(const CacheRowsCall& c, cudaStream_t st) { return rows_launch<false>(c, st); }
+
+uint32_t kv_cache_read_status(bool clear) {
+  uint32_t v = 0;
+  cudaMemcpyFromSymbol(&v, g_kv_cache_status, sizeof(v));
+  if (clear) {
+    const uint32_t z = 0;
+    cudaMemcpyToSymbol(g_kv_cache_status, &z, sizeof(z));
+  }
+  return v;
+}
+
+}  // namespace b2
