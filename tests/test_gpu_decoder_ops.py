@@ -609,7 +609,9 @@ def test_packed_masked_values_do_not_reach_a_result(dtype, D, value):
     seen = torch.zeros_like(got, dtype=torch.bool)
     seen[:70] = True
     seen[70 + 150:270, 2:, 5] = True
-    assert torch.equal(got[~seen], clean[~seen])
+    # a row beside a poisoned key may be summed in another order than in the clean run
+    tol = 1e-4 if dtype == torch.float32 else (U[dtype] + 3e-4) * v.abs().max().double().item()
+    check(got[~seen], clean[~seen], 2 * tol, dtype)
     want = torch.full_like(got[70 + 150:270, 2:, 5], value)
     assert torch.equal(torch.isnan(got[220:270, 2:, 5]), torch.isnan(want))
     if not math.isnan(value):

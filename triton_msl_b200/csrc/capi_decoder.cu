@@ -94,7 +94,7 @@ int cache_rows(const char* fn, bool write, CacheRowsCall& c, const int64_t cache
 
 uint32_t decoder_read_status(bool clear) {
   return rope_read_status(clear) | kv_cache_read_status(clear) | kv_cache_attn_read_status(clear) |
-         fa_packed_simt_read_status(clear);
+         fa_packed_read_status(clear) | fa_packed_simt_read_status(clear);
 }
 
 }  // namespace b2
@@ -227,8 +227,10 @@ int b2_fa_packed(const void* q, const void* k, const void* v, void* o, const int
   }
   const PackedCall c = {q, k, v, o, cu_q, cu_k, B, Tq, Tk, Hq, Hk, D, strides, sm_scale,
                         causal ? 1 : 0, dtype, workspace, ws_bytes};
-  const int rc = fa_packed_simt_launch(c, reinterpret_cast<cudaStream_t>(stream));
-  if (rc == B2_OK) set_last_kernel("fa_packed_simt");
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool tensor = device_is_sm100() && fa_packed_sm100_eligible(c);
+  const int rc = tensor ? fa_packed_sm100_launch(c, st) : fa_packed_simt_launch(c, st);
+  if (rc == B2_OK) set_last_kernel(tensor ? "fa_packed_sm100" : "fa_packed_simt");
   return rc;
 }
 

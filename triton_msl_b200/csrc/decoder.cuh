@@ -75,6 +75,9 @@ struct PackedCall {
   size_t ws_bytes;
 };
 size_t fa_packed_workspace(int64_t B, int64_t Tq, int64_t share);
+bool fa_packed_sm100_eligible(const PackedCall& c);
+int fa_packed_sm100_launch(const PackedCall& c, cudaStream_t st);
+uint32_t fa_packed_read_status(bool clear);
 int fa_packed_simt_launch(const PackedCall& c, cudaStream_t st);
 uint32_t fa_packed_simt_read_status(bool clear);
 

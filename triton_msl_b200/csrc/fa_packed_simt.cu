@@ -180,8 +180,6 @@ int fa_packed_simt_launch(const PackedCall& c, cudaStream_t st) {
   }
 }
 
-size_t fa_packed_workspace(int64_t, int64_t, int64_t) { return 0; }
-
 uint32_t fa_packed_simt_read_status(bool clear) {
   uint32_t v = 0;
   cudaMemcpyFromSymbol(&v, g_packed_simt_status, sizeof(v));
