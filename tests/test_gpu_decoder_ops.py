@@ -362,7 +362,8 @@ def attn_check(q, cache, table, lens, scale=None, kernel=None):
 def test_cache_attn(dtype, lens, N, Hq, H, D, group, page):
     g = gen(sum(lens) + N + Hq)
     cache, table = filled(g, lens, H, D, group, page)
-    attn_check(randn(g, len(lens), N, Hq, D).to(dtype), cache, table, lens)
+    attn_check(randn(g, len(lens), N, Hq, D).to(dtype), cache, table, lens,
+               kernel="kv_attn_row" if dtype == torch.float32 else "kv_attn_mma")
 
 
 def test_cache_attn_many_sequences():
@@ -564,7 +565,8 @@ def test_packed(dtype, causal, lens, Hq, Hk, D):
     g = gen(sum(lens) + Hq + D)
     T = sum(lens)
     qkv = randn(g, T, Hq + 2 * Hk, D).to(dtype)
-    packed_check(qkv[:, :Hq], qkv[:, Hq:Hq + Hk], qkv[:, Hq + Hk:], lens, causal=causal)
+    packed_check(qkv[:, :Hq], qkv[:, Hq:Hq + Hk], qkv[:, Hq + Hk:], lens, causal=causal,
+                 kernel="fa_packed_simt" if dtype == torch.float32 else "fa_packed_sm100")
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])

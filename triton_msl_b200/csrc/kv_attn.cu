@@ -5,11 +5,13 @@
 // for the rows r = (n, head); L counts the new tokens, which are in the cache
 // already. A row without a key gives zeros.
 //
-// This kernel: one CTA per row, one warp per key in turn, each lane D/32
-// channels, the running maximum and sum of the softmax per warp and one merge
-// at the end. It reads a key head once per query head and serves fp32 queries.
+// fp16 and bf16 queries run kv_attn_mma.cu. The kernel here serves fp32 queries:
+// one CTA per row, one warp per key in turn, each lane D/32 channels, the running
+// maximum and sum of the softmax per warp and one merge at the end. It reads a key
+// head once per query head.
 #include "b2_common.cuh"
 #include "decoder.cuh"
+#include "kv_attn.cuh"
 
 namespace b2 {
 namespace {
@@ -18,17 +20,6 @@ __device__ uint32_t g_kv_attn_status;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowWarps = 4;
-
-struct AttnArgs {
-  const void* q;
-  void* o;
-  const uint8_t *k_codes, *v_codes;
-  const uint32_t *k_scales, *v_scales;
-  const int32_t *page_table, *lengths;
-  long long qb, qn, qh, ob, on, oh, table_stride;
-  int N, Hq, H, page_size, num_pages, max_pages;
-  float scale_log2;
-};
 
 template <typename T, int D, int GROUP>
 __global__ void __launch_bounds__(kRowWarps * 32) kv_attn_row_kernel(const __grid_constant__ AttnArgs a) {
@@ -119,7 +110,10 @@ int launch_row_typed(const AttnArgs& a, const CacheShape& s, long long rows, cud
 
 }  // namespace
 
-size_t kv_cache_attn_workspace(int64_t, int64_t, int64_t, int64_t) { return 0; }
+size_t kv_cache_attn_workspace(int64_t B, int64_t rows, int64_t kv_heads, int64_t D) {
+  if (B <= 0 || rows <= 0 || kv_heads <= 0 || (D != 64 && D != 128)) return 0;
+  return kv_attn_mma_workspace(rows, D);
+}
 
 int kv_cache_attn_launch(const CacheAttnCall& c, cudaStream_t st, const char** kernel) {
   const CacheShape& s = c.shape;
@@ -139,13 +133,30 @@ int kv_cache_attn_launch(const CacheAttnCall& c, cudaStream_t st, const char** k
   a.on = c.strides[4];
   a.oh = c.strides[5];
   a.table_stride = c.table_stride;
+  a.B = (int)c.B;
   a.N = (int)c.N;
   a.Hq = (int)c.Hq;
   a.H = (int)s.H;
+  a.G = (int)(c.Hq / s.H);
+  a.rows = (int)(c.N * a.G);
   a.page_size = (int)s.page_size;
   a.num_pages = (int)s.pages;
   a.max_pages = (int)c.max_pages;
   a.scale_log2 = c.sm_scale * kLog2e;
+  B2_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(&a.status), g_kv_attn_status));
+  // fp32 queries would lose bits as fp16 operands; a cache without pages has
+  // nothing that the other kernel could load in place of a page that is not there
+  if (c.dtype != B2_F32 && s.pages > 0) {
+    const size_t need = kv_attn_mma_workspace(a.rows, s.D);
+    if (!c.workspace || c.ws_bytes < need || (reinterpret_cast<uintptr_t>(c.workspace) & 15)) {
+      set_error("b2_kv_cache_attn: needs a 16-byte aligned workspace of %zu bytes", need);
+      return B2_EINVAL;
+    }
+    a.partials = static_cast<float*>(c.workspace);
+    a.q_vec = (reinterpret_cast<uintptr_t>(c.q) & 15) == 0 && a.qb % 8 == 0 && a.qn % 8 == 0 && a.qh % 8 == 0;
+    *kernel = "kv_attn_mma";
+    return kv_attn_mma_launch(a, (int)s.D, (int)s.group, c.dtype, st);
+  }
   const long long rows = c.B * c.N * c.Hq;
   *kernel = "kv_attn_row";
   switch (c.dtype) {
