@@ -18,18 +18,20 @@
 // (token, head) pairs that share a key head: a key is read once for all of them.
 //
 // Work is split along the keys: all sequences' tiles of 128 keys form one line that
-// is cut evenly among the CTAs (two per SM), whatever the lengths. Inside a tile
-// each of 8 warps takes 16 keys. A warp's codes and scales come by cp.async into its
-// own ring of shared memory, kStages deep, so no barrier is needed in the loop. At a
-// sequence's end, or the CTA's, the warps' partial results are merged; a sequence
-// cut between CTAs is joined by kv_attn_join_kernel from partials in the workspace,
-// in the order of the keys.
+// is cut evenly among the CTAs (four per SM), whatever the lengths. Inside a tile
+// each of 4 warps takes 32 keys in two steps. A warp's codes and scales come by
+// cp.async into its own two buffers of shared memory, so no barrier is needed in the
+// loop. At a sequence's end, or the CTA's, the warps' partial results are merged; a
+// sequence cut between CTAs is joined by kv_attn_join_kernel from partials in the
+// workspace, in the order of the keys.
 //
 // Softmax: the running maximum of a row is only raised when a score passes it by 2^8
 // (one vote a step), P = 2^(s - m) then stays below 2^8. P * sv is rounded to fp16
 // (the one rounding of weights, 2^-11); F, a power of two per warp, keeps sv * F
-// within [.., 64] so that the product stays in fp16's range. Scores, sums, the lowest
+// at 8 or below so that the product stays in fp16's range. Scores, sums, the lowest
 // values' part and the accumulators are fp32.
+#include <type_traits>
+
 #include "b2_common.cuh"
 #include "decoder.cuh"
 #include "kv_attn.cuh"
@@ -37,8 +39,11 @@
 namespace b2 {
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps, kStages = 4;
-constexpr int kTile = 16 * kWarps;  // keys
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 2;
+constexpr int kSteps = 2;                    // of 16 keys a warp and tile
+constexpr int kTile = 16 * kSteps * kWarps;  // keys
+// Maximum of no scores: any score passes it, and -inf minus it is -inf.
+constexpr float kNoMax = -3e38f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -122,11 +127,11 @@ __device__ __forceinline__ int tiles_of(const AttnArgs& a, int b) { return (keys
 __device__ __forceinline__ int row_token(const AttnArgs& a, int row) { return row / a.G; }
 
 template <typename T, int D, int GROUP, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(const __grid_constant__ AttnArgs a) {
   using R = Ring<D, GROUP>;
   constexpr int NG = R::NG, N64 = D / 64, WPT = D / 32, ROWS = 8 * NT;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* s_o = reinterpret_cast<float*>(smem + kWarps * kStages * R::kStage);  // [warp][row][D + 4]
+  float* s_o = reinterpret_cast<float*>(smem + kWarps * kStages * kSteps * R::kStage);  // [warp][row][D + 4]
   float* s_m = s_o + kWarps * ROWS * (D + 4);                                  // [warp][row]
   float* s_l = s_m + kWarps * ROWS;
   __shared__ Pair s_sum[kWarps];
@@ -175,95 +180,76 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
     __syncthreads();
   }
 
-  // A place on the line: sequence, segment (key head and row block), tile.
-  struct Cursor {
-    int b, seg, tile, tiles, keys;
-  };
-  auto settle = [&](Cursor& c) {  // at the end of a segment: to the next one that has tiles
-    if (c.tile < c.tiles) return;
-    c.tile = 0;
-    if (++c.seg < segs) return;
-    c.seg = 0;
-    do {
-      if (++c.b >= a.B) {
-        c.tiles = 0;
-        return;
-      }
-      c.keys = keys_of(a, c.b);
-      c.tiles = (c.keys + kTile - 1) / kTile;
-    } while (c.tiles == 0);
-  };
-  Cursor at;
-  at.b = s_seq;
-  at.keys = keys_of(a, at.b);
-  at.tiles = (at.keys + kTile - 1) / kTile;
-  at.seg = (int)((begin - s_first) / at.tiles);
-  at.tile = (int)((begin - s_first) - (long long)at.seg * at.tiles);
+  // The segment at hand: sequence, key head and block of rows.
+  struct Segment {
+    int b, kvh, rb, keys, tiles;
+  } sg;
+  sg.b = s_seq;
+  sg.keys = keys_of(a, sg.b);
+  sg.tiles = (sg.keys + kTile - 1) / kTile;
+  int tile;  // its first tile here
+  {
+    const int seg = (int)((begin - s_first) / sg.tiles);
+    sg.kvh = seg / a.row_blocks;
+    sg.rb = seg - sg.kvh * a.row_blocks;
+    tile = (int)((begin - s_first) - (long long)seg * sg.tiles);
+  }
+  int left = (int)(end - begin);  // tiles of this CTA
 
-  // ---- loads, kStages - 1 tiles ahead
-  uint8_t* ring = smem + warp * (kStages * R::kStage);
+  // ---- loads, one tile ahead
+  uint8_t* ring = smem + warp * (kStages * kSteps * R::kStage);
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
-  const int cpp = a.page_size / 16;  // chunks per page
-  Cursor ld = at;
-  long long ld_pos = begin;
-  int ld_page = 0, ld_off = 0;
-  bool ld_has = false;
-  unsigned bad_stages = 0;  // a stage whose page lies outside the cache
-  auto ld_lookup = [&] {    // the page of this warp's 16 keys of the tile; used one step later
-    const int chunk = ld.tile * kWarps + warp;
-    ld_has = ld_pos < end && chunk * 16 < ld.keys;
-    if (ld_has) {
-      const int idx = chunk / cpp;
-      ld_off = chunk - idx * cpp;
-      ld_page = a.page_table[ld.b * a.table_stride + idx];
+  const uint32_t page_rows = (uint32_t)a.H * a.page_size;
+  constexpr int kSegs = D / 32;  // 16-byte pieces of a row of codes
+  constexpr int kPieces = R::kScales / 16;
+  const uint32_t v_dst = R::kVCodes + v_place<D>(lane / kSegs, lane % kSegs);
+  const bool s_lane = lane < 2 * kPieces;  // lanes that load scales: first the keys', then the values'
+  const uint32_t s_dst = (lane < kPieces ? R::kKScales : R::kVScales) + (lane % kPieces) * 16;
+  const uint8_t *k_src, *v_src, *s_src;  // the segment's head in page 0, and this lane's piece
+  const int32_t* pages;                  // the sequence's row of the page table
+  int page[kSteps];                      // of the tile to be loaded next
+  bool wrong = false;                    // a page of the segment lies outside the cache
+  auto lookup = [&](int tl) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int key = tl * kTile + (warp * kSteps + s) * 16;
+      if (key < sg.keys) page[s] = pages[a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size];
     }
   };
-  auto ld_issue = [&](int stage) {
-    if (ld_has) {
-      const bool bad = ld_page < 0 || ld_page >= a.num_pages;
-      bad_stages = (bad_stages & ~(1u << stage)) | ((bad ? 1u : 0u) << stage);
-      const int kvh = ld.seg / a.row_blocks;
-      const size_t row = ((size_t)(bad ? 0 : ld_page) * a.H + kvh) * a.page_size + ld_off * 16;
-      const uint8_t* kc = a.k_codes + row * (D / 2);
-      const uint8_t* vc = a.v_codes + row * (D / 2);
-      const uint32_t dst = ring_addr + stage * R::kStage;
+  auto load = [&](int tl, int stage) {
 #pragma unroll
-      for (int i = 0; i < R::kCodes / 512; ++i) {
-        const int piece = i * 32 + lane;
-        cp_async16(dst + piece * 16, kc + piece * 16);
-        constexpr int kSegs = D / 32;  // 16-byte pieces of a row
-        cp_async16(dst + R::kVCodes + v_place<D>(piece / kSegs, piece % kSegs), vc + piece * 16);
-      }
-      constexpr int kPieces = R::kScales / 16;
-      if (lane < 2 * kPieces) {
-        const int p = lane % kPieces;
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(lane < kPieces ? a.k_scales : a.v_scales) + row * (NG * 4);
-        cp_async16(dst + (lane < kPieces ? R::kKScales : R::kVScales) + p * 16, src + p * 16);
+    for (int s = 0; s < kSteps; ++s) {
+      const int key = tl * kTile + (warp * kSteps + s) * 16;
+      if (key < sg.keys) {
+        const bool bad = (unsigned)page[s] >= (unsigned)a.num_pages;
+        wrong |= bad;
+        const uint32_t in_page = a.page_shift >= 0 ? key & (a.page_size - 1) : key % a.page_size;
+        const size_t row = (size_t)(bad ? 0u : (unsigned)page[s]) * page_rows + in_page;
+        const uint8_t* kc = k_src + row * (D / 2);
+        const uint8_t* vc = v_src + row * (D / 2);
+        const uint32_t dst = ring_addr + (stage * kSteps + s) * R::kStage;
+#pragma unroll
+        for (int i = 0; i < R::kCodes / 512; ++i) {
+          cp_async16(dst + lane * 16 + i * 512, kc + i * 512);
+          cp_async16(dst + v_dst + i * 512, vc + i * 512);  // 8 rows further: the same place, 512 bytes on
+        }
+        if (s_lane) cp_async16(dst + s_dst, s_src + row * (NG * 4));
       }
     }
     cp_async_commit();
-    if (ld_pos < end) {
-      ++ld_pos;
-      ++ld.tile;
-      settle(ld);
-      ld_lookup();
-    }
   };
-  ld_lookup();
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) ld_issue(s);
 
   // ---- a segment's state
   uint32_t qf[NT][WPT][2][2];          // B operands: code word, low or high byte pair, register
   float f[NT][2], qs[NT][NG][2];       // per column: factor of the code part, scaled sums of q
   int lim[NT][2];                      // keys each column's row keeps
-  float m[NT][2], mu[NT][2], l[NT][2], lo[NT][NG][2];
+  float m[NT][2], l[NT][2], lo[NT][NG][2];  // running maximum, sums
   float o[N64 * 4][NT][4];
   float F = 0.f;
   int keys_all = 0;                    // keys that every row keeps
 
-  auto begin_segment = [&](const Cursor& c) {
-    const int kvh = c.seg / a.row_blocks, rb = c.seg - kvh * a.row_blocks;
+  auto begin_segment = [&](const Segment& c) {
+    const int kvh = c.kvh, rb = c.rb;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = rb * ROWS + nt * 8 + g;
@@ -338,8 +324,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
         const int r = rb * ROWS + nt * 8 + 2 * t + c2;
         // rows that do not exist keep what the last token keeps
         lim[nt][c2] = r < a.rows ? max(0, c.keys - a.N + 1 + row_token(a, r)) : c.keys;
-        m[nt][c2] = -INFINITY;
-        mu[nt][c2] = 0.f;
+        m[nt][c2] = kNoMax;
         l[nt][c2] = 0.f;
 #pragma unroll
         for (int k = 0; k < NG; ++k) lo[nt][k][c2] = 0.f;
@@ -353,25 +338,31 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
     keys_all = max(0, c.keys - a.N + 1);
   };
 
+  const int k_off = g * (D / 2) + t * (D / 8), m_off = R::kKScales + g * NG * 4;
+  const int v_off = R::kVCodes + v_place<D>(2 * t, D == 128 ? g >> 1 : g >> 2) + (D == 128 ? (g & 1) * 8 : (g & 3) * 4);
+
   // ---- 16 keys
-  auto step = [&](const uint8_t* st, int key0, int keys, bool bad) {
+  auto step = [&](const uint8_t* st, int key0, int keys) {
     // scores
-    uint32_t k0[WPT], k1[WPT];
+    uint32_t k0[WPT], k1[WPT], km[2][NG], vm[2][NG];
     if constexpr (D == 128) {
-      *reinterpret_cast<uint4*>(k0) = *reinterpret_cast<const uint4*>(st + g * 64 + t * 16);
-      *reinterpret_cast<uint4*>(k1) = *reinterpret_cast<const uint4*>(st + (g + 8) * 64 + t * 16);
+      *reinterpret_cast<uint4*>(k0) = *reinterpret_cast<const uint4*>(st + k_off);
+      *reinterpret_cast<uint4*>(k1) = *reinterpret_cast<const uint4*>(st + k_off + 8 * (D / 2));
     } else {
-      *reinterpret_cast<uint2*>(k0) = *reinterpret_cast<const uint2*>(st + g * 32 + t * 8);
-      *reinterpret_cast<uint2*>(k1) = *reinterpret_cast<const uint2*>(st + (g + 8) * 32 + t * 8);
+      *reinterpret_cast<uint2*>(k0) = *reinterpret_cast<const uint2*>(st + k_off);
+      *reinterpret_cast<uint2*>(k1) = *reinterpret_cast<const uint2*>(st + k_off + 8 * (D / 2));
     }
-    uint32_t km[2][NG], vm[2][NG];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        km[h][k] = *reinterpret_cast<const uint32_t*>(st + R::kKScales + ((g + 8 * h) * NG + k) * 4);
-        vm[h][k] = *reinterpret_cast<const uint32_t*>(st + R::kVScales + ((g + 8 * h) * NG + k) * 4);
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* p = st + m_off + 8 * h * NG * 4;
+      if constexpr (NG == 2) {
+        *reinterpret_cast<uint2*>(km[h]) = *reinterpret_cast<const uint2*>(p);
+        *reinterpret_cast<uint2*>(vm[h]) = *reinterpret_cast<const uint2*>(p + R::kScales);
+      } else {
+        km[h][0] = *reinterpret_cast<const uint32_t*>(p);
+        vm[h][0] = *reinterpret_cast<const uint32_t*>(p + R::kScales);
       }
+    }
     float acc[NG][NT][4] = {};
 #pragma unroll
     for (int w = 0; w < WPT; ++w)
@@ -397,12 +388,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int h = i >> 1, c2 = i & 1;
-        float x = scale_of(km[h][0]) * acc[0][nt][i], y = low_of(km[h][0]) * qs[nt][0][c2];
+        float u = scale_of(km[h][0]) * acc[0][nt][i], y = low_of(km[h][0]) * qs[nt][0][c2];
         if constexpr (NG == 2) {
-          x = fmaf(scale_of(km[h][1]), acc[1][nt][i], x);
+          u = fmaf(scale_of(km[h][1]), acc[1][nt][i], u);
           y = fmaf(low_of(km[h][1]), qs[nt][1][c2], y);
         }
-        sc[nt][i] = fmaf(x, f[nt][c2], y);
+        sc[nt][i] = fmaf(u, f[nt][c2], y);
       }
     const bool edge = key0 + 16 > keys_all;  // some row keeps only a part
     if (edge) {
@@ -421,21 +412,32 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
       }
     }
     // raise the maxima, or lower F, where needed
-    bool raise = false;
+    float x[NT][4], svf[2][NG];
+    auto relative = [&] {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[nt][i] = sc[nt][i] - m[nt][i & 1];
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        svf[0][k] = sv[0][k] * F;
+        svf[1][k] = sv[1][k] * F;
+      }
+    };
+    relative();
+    float over = fmaxf(svf[0][0], svf[1][0]);
+    if constexpr (NG == 2) over = fmaxf(over, fmaxf(svf[0][1], svf[1][1]));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c2 = 0; c2 < 2; ++c2) raise = raise || fmaxf(sc[nt][c2], sc[nt][2 + c2]) > m[nt][c2] + 8.f;
-#pragma unroll
-    for (int k = 0; k < NG; ++k) raise = raise || fmaxf(sv[0][k], sv[1][k]) * F > 64.f;
-    if (__any_sync(0xffffffffu, raise)) {
+      over = fmaxf(over, fmaxf(fmaxf(x[nt][0], x[nt][1]), fmaxf(x[nt][2], x[nt][3])));
+    if (__any_sync(0xffffffffu, over > 8.f)) {
       float top = 0.f;
 #pragma unroll
       for (int k = 0; k < NG; ++k) top = fmaxf(top, fmaxf(sv[0][k], sv[1][k]));  // NaN is left aside
       const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
       float ratio = 1.f;
-      if (__uint_as_float(top_bits) * F > 64.f) {
-        const float to = __int_as_float(min(max(259 - (int)(top_bits >> 23), 1), 254) << 23);
+      if (__uint_as_float(top_bits) * F > 8.f) {  // to 4 .. 8
+        const float to = __int_as_float(min(max(256 - (int)(top_bits >> 23), 1), 254) << 23);
         ratio = to / F;
         F = to;
       }
@@ -443,14 +445,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c2 = 0; c2 < 2; ++c2) {
-          float x = fmaxf(sc[nt][c2], sc[nt][2 + c2]);
+          float y = fmaxf(sc[nt][c2], sc[nt][2 + c2]);
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-          const float to = fmaxf(m[nt][c2], x);
-          const float base = to == -INFINITY ? 0.f : to;
-          const float al = ex2(m[nt][c2] - base);
+          for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+          const float to = fmaxf(m[nt][c2], y);
+          const float al = ex2(m[nt][c2] - to);
           m[nt][c2] = to;
-          mu[nt][c2] = base;
           l[nt][c2] *= al;
 #pragma unroll
           for (int k = 0; k < NG; ++k) lo[nt][k][c2] *= al;
@@ -460,62 +460,71 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
             o[i][nt][2 + c2] *= al * ratio;
           }
         }
+      relative();
     }
     // weights, and their products with the values' scales as the B operand
+    // F is a power of two: 1/F by its exponent
+    const float mid = 7.5f * __int_as_float((254 << 23) - __float_as_int(F));
     uint32_t pf[NT][NG][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float p[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[i] = ex2(sc[nt][i] - mu[nt][i & 1]);
+        p[i] = ex2(x[nt][i]);
         l[nt][i & 1] += p[i];
       }
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = p[i] * (sv[i >> 1][k] * F);
-        float y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = p[i] * lv[i >> 1][k];
+        for (int i = 0; i < 4; ++i) w[i] = p[i] * svf[i >> 1][k];
         if (edge) {
           // a row's own masked keys count for nothing, NaN or not
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (key0 + g + 8 * (i >> 1) >= lim[nt][i & 1]) w[i] = y[i] = 0.f;
+          for (int i = 0; i < 4; ++i) {
+            const bool out = key0 + g + 8 * (i >> 1) >= lim[nt][i & 1];
+            if (out) w[i] = 0.f;
+            lo[nt][k][i & 1] += out ? 0.f : p[i] * lv[i >> 1][k];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) lo[nt][k][i & 1] = fmaf(p[i], lv[i >> 1][k], lo[nt][k][i & 1]);
         }
-        lo[nt][k][0] += y[0] + y[2];
-        lo[nt][k][1] += y[1] + y[3];
-        pf[nt][k][0] = transpose8(half2_bits(w[0], w[1]));
-        pf[nt][k][1] = transpose8(half2_bits(w[2], w[3]));
+        uint32_t packed[2] = {half2_bits(w[0], w[1]), half2_bits(w[2], w[3])};
+        if constexpr (std::is_same<T, __half>::value) {
+          // What the rounding took from a weight, times the middle of the codes, goes
+          // to the lowest values' sum: the rounding then counts for the code's distance
+          // from 7.5 and not for the whole code. fp16 results resolve that (error of 16
+          // sequences of up to 4095 keys 4.5e-4 -> MEASURE); bf16 ones do not.
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&packed[h]));
+            lo[nt][k][0] = fmaf(w[2 * h] - r.x, mid, lo[nt][k][0]);
+            lo[nt][k][1] = fmaf(w[2 * h + 1] - r.y, mid, lo[nt][k][1]);
+          }
+        }
+        pf[nt][k][0] = transpose8(packed[0]);
+        pf[nt][k][1] = transpose8(packed[1]);
       }
-    }
-    if (bad) {  // no such page: every row that reaches it is undefined
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c2 = 0; c2 < 2; ++c2)
-          if (key0 < lim[nt][c2]) l[nt][c2] = __int_as_float(0x7fffffff);
     }
     // values
+    uint32_t vw[4][N64];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // keys 2t + (i & 1) + 8 (i >> 1): v_place keeps their distances
+      const uint8_t* p = st + v_off + ((i & 1) * 4 + (i >> 1) * 8) * (D / 2);
+      if constexpr (D == 128) *reinterpret_cast<uint2*>(vw[i]) = *reinterpret_cast<const uint2*>(p);
+      else vw[i][0] = *reinterpret_cast<const uint32_t*>(p);
+    }
 #pragma unroll
     for (int w = 0; w < N64; ++w) {
-      uint32_t x[4];  // keys 2t, 2t+1, 2t+8, 2t+9: channels 64w + 8g ..
+      uint32_t y[4];  // keys 2t, 2t+1, 2t+8, 2t+9: channels 64w + 8g ..
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 2 * t + (i & 1) + 8 * (i >> 1);
-        if constexpr (D == 128) {
-          const uint2 y = *reinterpret_cast<const uint2*>(st + R::kVCodes + v_place<D>(row, g >> 1) + (g & 1) * 8);
-          x[i] = w ? y.y : y.x;
-        } else {
-          x[i] = *reinterpret_cast<const uint32_t*>(st + R::kVCodes + v_place<D>(row, g >> 2) + (g & 3) * 4);
-        }
-      }
+      for (int i = 0; i < 4; ++i) y[i] = vw[i][w];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // codes 4h .. 4h+3 of each word
-        uint32_t p0 = __byte_perm(x[0], x[1], h ? 0x7632 : 0x5410);
-        uint32_t p1 = __byte_perm(x[2], x[3], h ? 0x7632 : 0x5410);
+        uint32_t p0 = __byte_perm(y[0], y[1], h ? 0x7632 : 0x5410);
+        uint32_t p1 = __byte_perm(y[2], y[3], h ? 0x7632 : 0x5410);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const uint32_t a0 = p0 & 0x000f000fu, a1 = p0 & 0x00f000f0u;
@@ -531,8 +540,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
   };
 
   // ---- merge the warps' results of a segment
-  auto end_segment = [&](const Cursor& c, long long seg_begin) {
-    const int kvh = c.seg / a.row_blocks, rb = c.seg - kvh * a.row_blocks;
+  auto end_segment = [&](const Segment& c, long long seg_begin) {
+    const int kvh = c.kvh, rb = c.rb;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -543,12 +552,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
 #pragma unroll
           for (int k = 0; k < NG; ++k) lo[nt][k][c2] += __shfl_xor_sync(0xffffffffu, lo[nt][k][c2], d);
         }
+        if (wrong) l[nt][c2] = __int_as_float(0x7fffffff);  // no such page: the rows are undefined
         const int r = nt * 8 + 2 * t + c2;
         if (g == 0) {
           s_m[warp * ROWS + r] = m[nt][c2];
           s_l[warp * ROWS + r] = l[nt][c2];
         }
-        const float down = 1.f / F;  // a power of two, in range; 2^24 / F need not be
+        const float down = 1.f / F;  // in range; 2^24 / F need not be
 #pragma unroll
         for (int i = 0; i < N64 * 4; ++i) {
           const int d = 64 * (i / 4) + 8 * g + 2 * (i % 4);
@@ -565,15 +575,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
     for (int e = threadIdx.x; e < ROWS * (D / 4); e += kThreads) {
       const int r = e / (D / 4), d = (e % (D / 4)) * 4;
       const int row = rb * ROWS + r;
-      float top = -INFINITY;
+      float top = kNoMax;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w * ROWS + r]);
-      const float base = top == -INFINITY ? 0.f : top;
       float sum = 0.f;
       float4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float x = ex2(s_m[w * ROWS + r] - base);
+        const float x = ex2(s_m[w * ROWS + r] - top);
         const float4 y = *reinterpret_cast<const float4*>(s_o + (w * ROWS + r) * (D + 4) + d);
         sum = fmaf(x, s_l[w * ROWS + r], sum);
         v.x = fmaf(x, y.x, v.x);
@@ -603,118 +612,166 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv_attn_kernel(cons
     __syncthreads();
   };
 
-  // ---- the line
-  long long seg_begin = begin - at.tile;  // of the segment at hand
-  begin_segment(at);
-  int stage = 0;
-  for (long long pos = begin; pos < end; ++pos) {
-    cp_async_wait<kStages - 2>();
-    __syncwarp();  // the other lanes' pieces have landed, and all are done with the oldest stage
-    const bool bad = (bad_stages >> stage) & 1;  // before the next issue reuses the bit
-    ld_issue((stage + kStages - 1) % kStages);
-    const int key0 = (at.tile * kWarps + warp) * 16;
-    if (key0 < at.keys) {
-      if (bad && lane == 0) atomicOr(a.status, DEV_BAD_INDEX);
-      step(ring + stage * R::kStage, key0, at.keys, bad);
+  // ---- the segments of this CTA's part of the line
+  long long pos = begin;
+  while (true) {
+    const long long seg_begin = pos - tile;
+    const int stop = min(sg.tiles, tile + left);
+    {
+      const size_t head = (size_t)sg.kvh * a.page_size;
+      k_src = a.k_codes + head * (D / 2) + lane * 16;
+      v_src = a.v_codes + head * (D / 2) + lane * 16;
+      s_src = reinterpret_cast<const uint8_t*>(lane < kPieces ? a.k_scales : a.v_scales) + head * (NG * 4) + (lane % kPieces) * 16;
+      pages = a.page_table + sg.b * a.table_stride;
     }
-    stage = (stage + 1) % kStages;
-    const bool last = at.tile + 1 == at.tiles;
-    if (last || pos + 1 == end) {
-      end_segment(at, seg_begin);
-      if (pos + 1 < end) {
-        seg_begin = pos + 1;
-        ++at.tile;
-        settle(at);
-        begin_segment(at);
+    wrong = false;
+    left -= stop - tile;
+    pos += stop - tile;
+    lookup(tile);
+    load(tile, 0);
+    if (tile + 1 < stop) lookup(tile + 1);
+    begin_segment(sg);
+    int stage = 0;
+    for (; tile < stop; ++tile) {
+      cp_async_wait<0>();
+      __syncwarp();  // the other lanes' pieces have landed, and all are done with the other buffer
+      if (tile + 1 < stop) {
+        load(tile + 1, stage ^ 1);
+        if (tile + 2 < stop) lookup(tile + 2);
       }
-    } else {
-      ++at.tile;
+#pragma unroll 1
+      for (int s = 0; s < kSteps; ++s) {
+        const int key0 = tile * kTile + (warp * kSteps + s) * 16;
+        if (key0 >= sg.keys) break;
+        step(ring + (stage * kSteps + s) * R::kStage, key0, sg.keys);
+      }
+      stage ^= 1;
+    }
+    if (wrong && lane == 0) atomicOr(a.status, DEV_BAD_INDEX);
+    end_segment(sg, seg_begin);
+    if (left == 0) break;
+    // the next segment that has tiles
+    tile = 0;
+    if (++sg.rb == a.row_blocks) {
+      sg.rb = 0;
+      if (++sg.kvh == a.H) {
+        sg.kvh = 0;
+        do {
+          if (++sg.b >= a.B) return;
+          sg.keys = keys_of(a, sg.b);
+          sg.tiles = (sg.keys + kTile - 1) / kTile;
+        } while (sg.tiles == 0);
+      }
     }
   }
-  cp_async_wait<0>();
 }
 
 // Joins the parts of the segments that were cut between CTAs; writes the rows of
-// sequences without tiles (no key, or a length that cannot be).
+// sequences without tiles (no key, or a length that cannot be). One CTA per row: its
+// threads take the row's channels four at a time and the parts kJoin / (D/4) at once.
+constexpr int kJoin = 128;
+constexpr int kJoinMax = 1024;  // parts whose weights are kept; a segment has at most the grid's CTAs
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kThreads) kv_attn_join_kernel(const __grid_constant__ AttnArgs a, long long grid) {
-  __shared__ Pair s_sum[kWarps];
-  const int segs = a.H * a.row_blocks;
-  const int b = blockIdx.x / segs, seg = blockIdx.x - b * segs;
-  const int kvh = seg / a.row_blocks, rb = seg - kvh * a.row_blocks;
-  const int tiles = tiles_of(a, b);
-  long long before = 0, total = 0;
-  if (tiles > 0) {
-    long long mine_before = 0, mine = 0;
-    for (int i = threadIdx.x; i < a.B; i += kThreads) {
-      const int n = tiles_of(a, i);
-      mine += n;
-      if (i < b) mine_before += n;
-    }
-    const Pair s = block_sum<kWarps>(mine, mine_before, s_sum);
-    total = s.a * segs;
-    before = s.b * segs + (long long)seg * tiles;
+__global__ void __launch_bounds__(kJoin) kv_attn_join_kernel(const __grid_constant__ AttnArgs a, int grid) {
+  constexpr int LANES = D / 4, LINES = kJoin / LANES;
+  __shared__ Pair s_sum[kJoin / 32];
+  __shared__ float s_w[kJoinMax], s_top[kJoin / 32], s_total[kJoin / 32];
+  __shared__ float4 s_v[LINES][LANES];
+  const int per_seq = a.H * a.rows;
+  const int b = blockIdx.x / per_seq, rest = blockIdx.x - b * per_seq;
+  const int kvh = rest / a.rows, row = rest - kvh * a.rows;
+  const int rb = row / ROWS, r = row - rb * ROWS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int segs = a.H * a.row_blocks, seg = kvh * a.row_blocks + rb;
+  const int held = a.lengths[b], tiles = tiles_of(a, b);
+  const int n = row_token(a, row);
+  T* out = static_cast<T*>(a.o) + (long long)b * a.ob + n * a.on + (long long)(kvh * a.G + row - n * a.G) * a.oh;
+  // every CTA waits for the attention kernel, so that this one's end is the call's
+  if (tiles == 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const bool wrong = held != 0;
+    if (wrong && threadIdx.x == 0) atomicOr(a.status, DEV_BAD_INDEX);
+    for (int d = threadIdx.x; d < D; d += kJoin) out[d] = from_f32<T>(wrong ? __int_as_float(0x7fffffff) : 0.f);
+    return;
   }
+  long long mine_before = 0, mine = 0;
+  for (int i = threadIdx.x; i < a.B; i += kJoin) {
+    const int k = tiles_of(a, i);
+    mine += k;
+    if (i < b) mine_before += k;
+  }
+  const Pair s = block_sum<kJoin / 32>(mine, mine_before, s_sum);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int held = a.lengths[b];
-  const bool wrong = tiles == 0 && held != 0;
-  long long c0 = 0, c1 = 0;
-  if (tiles > 0) {
-    const long long ctas = total < grid ? total : grid;
-    // CTA c holds tiles [c * total / ctas, (c + 1) * total / ctas)
-    c0 = ((before + 1) * ctas - 1) / total;
-    c1 = ((before + tiles) * ctas - 1) / total;
-    if (c0 == c1) return;  // whole in one CTA, which wrote it
-  } else if (wrong && threadIdx.x == 0) {
-    atomicOr(a.status, DEV_BAD_INDEX);
-  }
+  const long long total = s.a * segs, before = s.b * segs + (long long)seg * tiles;
+  const long long ctas = total < grid ? total : grid;
+  // CTA c holds tiles [c * total / ctas, (c + 1) * total / ctas)
+  const int c0 = (int)(((before + 1) * ctas - 1) / total), c1 = (int)(((before + tiles) * ctas - 1) / total);
+  if (c0 == c1) return;  // whole in one CTA, which wrote it
+  const int parts = c1 - c0 + 1;
+  // the first CTA's part began in it (slot 1), the others' began before them (slot 0)
   const size_t stride = (size_t)ROWS * (D + 2);
-  for (int e = threadIdx.x; e < ROWS * (D / 4); e += kThreads) {
-    const int r = e / (D / 4), d = (e % (D / 4)) * 4;
-    const int row = rb * ROWS + r;
-    if (row >= a.rows) continue;
-    const int n = row_token(a, row);
-    float4 v = {0.f, 0.f, 0.f, 0.f};
-    if (tiles > 0 && held - a.N + 1 + n > 0) {
-      // the first CTA's part began in it (slot 1), the others' began before them
-      auto part = [&](long long c) { return a.partials + (size_t)(2 * c + (c == c0 ? 1 : 0)) * stride; };
-      float top = -INFINITY;
-      for (long long c = c0; c <= c1; ++c) top = fmaxf(top, part(c)[ROWS * D + r]);
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-#pragma unroll 4
-      for (long long c = c0; c <= c1; ++c) {
-        const float* p = part(c);
-        const float x = ex2(p[ROWS * D + r] - base);
-        const float4 y = *reinterpret_cast<const float4*>(p + r * D + d);
-        sum = fmaf(x, p[ROWS * D + ROWS + r], sum);
-        v.x = fmaf(x, y.x, v.x);
-        v.y = fmaf(x, y.y, v.y);
-        v.z = fmaf(x, y.z, v.z);
-        v.w = fmaf(x, y.w, v.w);
-      }
-      v.x /= sum;
-      v.y /= sum;
-      v.z /= sum;
-      v.w /= sum;
-    } else if (wrong) {
-      v.x = v.y = v.z = v.w = __int_as_float(0x7fffffff);
+  auto part = [&](int i) { return a.partials + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * stride; };
+  float top = kNoMax;
+  for (int i = threadIdx.x; i < parts; i += kJoin) {
+    s_w[i] = part(i)[ROWS * D + r];
+    top = fmaxf(top, s_w[i]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoin / 32; ++w) top = fmaxf(top, s_top[w]);
+  float sum = 0.f;
+  for (int i = threadIdx.x; i < parts; i += kJoin) {
+    s_w[i] = ex2(s_w[i] - top);
+    sum = fmaf(s_w[i], part(i)[ROWS * D + ROWS + r], sum);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) s_total[warp] = sum;
+  __syncthreads();
+  const int col = threadIdx.x % LANES, line = threadIdx.x / LANES;
+  float4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int i = line; i < parts; i += LINES) {
+    const float4 y = *reinterpret_cast<const float4*>(part(i) + r * D + 4 * col);
+    const float w = s_w[i];
+    v.x = fmaf(w, y.x, v.x);
+    v.y = fmaf(w, y.y, v.y);
+    v.z = fmaf(w, y.z, v.z);
+    v.w = fmaf(w, y.w, v.w);
+  }
+  s_v[line][col] = v;
+  __syncthreads();
+  if (line == 0) {
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoin / 32; ++w) all += s_total[w];
+#pragma unroll
+    for (int i = 1; i < LINES; ++i) {
+      const float4 y = s_v[i][col];
+      v.x += y.x;
+      v.y += y.y;
+      v.z += y.z;
+      v.w += y.w;
     }
-    T* out = static_cast<T*>(a.o) + (long long)b * a.ob + n * a.on + (long long)(kvh * a.G + row - n * a.G) * a.oh + d;
-    out[0] = from_f32<T>(v.x);
-    out[1] = from_f32<T>(v.y);
-    out[2] = from_f32<T>(v.z);
-    out[3] = from_f32<T>(v.w);
+    const bool any = held - a.N + 1 + n > 0;
+    out[4 * col] = from_f32<T>(any ? v.x / all : 0.f);
+    out[4 * col + 1] = from_f32<T>(any ? v.y / all : 0.f);
+    out[4 * col + 2] = from_f32<T>(any ? v.z / all : 0.f);
+    out[4 * col + 3] = from_f32<T>(any ? v.w / all : 0.f);
   }
 }
 
-constexpr int kMaxGrid = 2 * 160;  // CTAs that the workspace has room for
+constexpr int kMaxGrid = 4 * 160;  // CTAs that the workspace has room for
+static_assert(kMaxGrid <= kJoinMax, "a segment's parts");
 
 template <typename T, int D, int GROUP, int NT>
 int launch(AttnArgs& a, cudaStream_t st) {
   using R = Ring<D, GROUP>;
   constexpr int ROWS = 8 * NT;
-  constexpr size_t smem = (size_t)kWarps * kStages * R::kStage + (size_t)kWarps * ROWS * (D + 6) * sizeof(float);
+  constexpr size_t smem = (size_t)kWarps * kStages * kSteps * R::kStage + (size_t)kWarps * ROWS * (D + 6) * sizeof(float);
   a.row_blocks = (a.rows + ROWS - 1) / ROWS;
   const long long segs = (long long)a.B * a.H * a.row_blocks;
   if (segs >= (1LL << 31)) {
@@ -723,7 +780,7 @@ int launch(AttnArgs& a, cudaStream_t st) {
   }
   auto kern = kv_attn_kernel<T, D, GROUP, NT>;
   B2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  int grid = device_sm_count() * (NT == 1 ? 2 : 1);
+  int grid = device_sm_count() * (NT == 1 ? 4 : 2);
   if (grid > kMaxGrid) grid = kMaxGrid;
   kern<<<grid, kThreads, smem, st>>>(a);
   B2_CHECK_LAUNCH();
@@ -731,19 +788,22 @@ int launch(AttnArgs& a, cudaStream_t st) {
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)segs);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)((long long)a.B * a.H * a.rows));
+  cfg.blockDim = dim3(kJoin);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  B2_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_attn_join_kernel<T, D, ROWS>, a, (long long)grid));
+  B2_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_attn_join_kernel<T, D, ROWS>, a, grid));
   return B2_OK;
 }
 
 template <typename T>
 int launch_typed(AttnArgs& a, int D, int group, cudaStream_t st) {
   const bool one = a.rows <= 8;
-  if (D == 64) return one ? launch<T, 64, 64, 1>(a, st) : launch<T, 64, 64, 2>(a, st);
+  if (D == 64) {
+    if (a.rows > 16) return launch<T, 64, 64, 4>(a, st);
+    return one ? launch<T, 64, 64, 1>(a, st) : launch<T, 64, 64, 2>(a, st);
+  }
   if (group == 64) return one ? launch<T, 128, 64, 1>(a, st) : launch<T, 128, 64, 2>(a, st);
   return one ? launch<T, 128, 128, 1>(a, st) : launch<T, 128, 128, 2>(a, st);
 }
@@ -751,7 +811,8 @@ int launch_typed(AttnArgs& a, int D, int group, cudaStream_t st) {
 }  // namespace
 
 size_t kv_attn_mma_workspace(int64_t rows, int64_t D) {
-  return sizeof(float) * 2 * kMaxGrid * (size_t)(rows <= 8 ? 8 : 16) * (size_t)(D + 2);
+  const size_t block = rows <= 8 ? 8 : rows <= 16 || D > 64 ? 16 : 32;
+  return sizeof(float) * 2 * kMaxGrid * block * (size_t)(D + 2);
 }
 
 int kv_attn_mma_launch(AttnArgs& a, int D, int group, int dtype, cudaStream_t st) {
