@@ -42,7 +42,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 2;
 constexpr int kSteps = 2;                    // of 16 keys a warp and tile
 constexpr int kTile = 16 * kSteps * kWarps;  // keys
-// Maximum of no scores: any score passes it, and -inf minus it is -inf.
+// Maximum of no scores.
 constexpr float kNoMax = -3e38f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -94,34 +94,46 @@ __device__ __forceinline__ int v_place(int row, int seg) {
   return r * (D / 2) + seg * 16;
 }
 
-// Sum over the CTA of two numbers per thread.
-struct Pair {
-  long long a, b;
-};
-template <int WARPS>
-__device__ __forceinline__ Pair block_sum(long long a, long long b, Pair* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = {a, b};
-  __syncthreads();
-  Pair s = {0, 0};
-  for (int w = 0; w < WARPS; ++w) {
-    s.a += scratch[w].a;
-    s.b += scratch[w].b;
-  }
-  return s;
-}
-
 // A sequence's keys: 0 when the length is not one the page table can hold.
 __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
   const int n = a.lengths[b];
   return n < 0 || n > (long long)a.max_pages * a.page_size ? 0 : n;
 }
 __device__ __forceinline__ int tiles_of(const AttnArgs& a, int b) { return (keys_of(a, b) + kTile - 1) / kTile; }
+
+// The line of all tiles: sequence after sequence, in each segment after segment (key
+// head, block of rows). CTA c of n holds tiles [share * c + min(c, more), ...).
+struct Line {
+  unsigned share, more, ctas;
+  __device__ Line(unsigned total, unsigned grid) {
+    ctas = min(total, grid);
+    share = ctas ? total / ctas : 0;
+    more = total - share * ctas;
+  }
+  __device__ unsigned begin(unsigned c) const { return share * c + min(c, more); }
+  __device__ unsigned owner(unsigned tile) const {
+    const unsigned big = more * (share + 1);
+    return tile < big ? tile / (share + 1) : more + (tile - big) / share;
+  }
+};
+// Tiles per segment of all sequences, and of those before b; the whole warp.
+__device__ __forceinline__ unsigned count_tiles(const AttnArgs& a, int b, unsigned* before) {
+  unsigned all = 0, some = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x & 31; i < a.B; i += 32) {
+    const unsigned n = tiles_of(a, i);
+    all += n;
+    if (i < b) some += n;
+  }
+  if (before) *before = __reduce_add_sync(0xffffffffu, some);
+  return __reduce_add_sync(0xffffffffu, all);
+}
+// 3-input maximum
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 
 // One row of the group: its token among the new ones and its query head.
 __device__ __forceinline__ int row_token(const AttnArgs& a, int row) { return row / a.G; }
@@ -134,65 +146,46 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
   float* s_o = reinterpret_cast<float*>(smem + kWarps * kStages * kSteps * R::kStage);  // [warp][row][D + 4]
   float* s_m = s_o + kWarps * ROWS * (D + 4);                                  // [warp][row]
   float* s_l = s_m + kWarps * ROWS;
-  __shared__ Pair s_sum[kWarps];
-  __shared__ int s_seq;
-  __shared__ long long s_first;
-
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int segs = a.H * a.row_blocks;  // lines of tiles per sequence
 
-  // ---- this CTA's part of the line of all tiles
+  // ---- this CTA's part of the line of all tiles; every warp finds it by itself
   asm volatile("griddepcontrol.launch_dependents;");
-  long long total = 0;
-  {
-    long long mine = 0;
-    for (int b = threadIdx.x; b < a.B; b += kThreads) mine += tiles_of(a, b);
-    total = block_sum<kWarps>(mine, 0, s_sum).a * segs;
-  }
-  const long long ctas = total < gridDim.x ? total : gridDim.x;
-  if (blockIdx.x >= ctas) return;
-  const long long begin = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
-  {
-    // the sequence that holds tile `begin`: prefix sums, kThreads sequences at a time
-    long long before = 0;
-    for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-      const int b = b0 + threadIdx.x;
-      const long long n = b < a.B ? (long long)tiles_of(a, b) * segs : 0;
-      long long inc = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      __syncthreads();
-      if (lane == 31) s_sum[warp] = {inc, 0};
-      __syncthreads();
-      long long base = before;
-      for (int w = 0; w < warp; ++w) base += s_sum[w].a;
-      if (n > 0 && begin >= base + inc - n && begin < base + inc) {
-        s_seq = b;
-        s_first = base + inc - n;
-      }
-      for (int w = 0; w < kWarps; ++w) before += s_sum[w].a;
-      if (before > begin) break;
-    }
-    __syncthreads();
-  }
-
+  const Line line(count_tiles(a, 0, nullptr) * segs, gridDim.x);
+  if (blockIdx.x >= line.ctas) return;
+  const unsigned begin = line.begin(blockIdx.x), end = line.begin(blockIdx.x + 1);
   // The segment at hand: sequence, key head and block of rows.
   struct Segment {
     int b, kvh, rb, keys, tiles;
-  } sg;
-  sg.b = s_seq;
-  sg.keys = keys_of(a, sg.b);
-  sg.tiles = (sg.keys + kTile - 1) / kTile;
-  int tile;  // its first tile here
+  } sg = {};
+  int tile = 0;  // its first tile here
   {
-    const int seg = (int)((begin - s_first) / sg.tiles);
-    sg.kvh = seg / a.row_blocks;
-    sg.rb = seg - sg.kvh * a.row_blocks;
-    tile = (int)((begin - s_first) - (long long)seg * sg.tiles);
+    unsigned base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int keys = b0 + lane < a.B ? keys_of(a, b0 + lane) : 0;
+      const unsigned n = (unsigned)((keys + kTile - 1) / kTile) * segs;
+      unsigned inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, begin < base + inc);
+      if (hit) {
+        const int w = __ffs(hit) - 1;
+        sg.b = b0 + w;
+        sg.keys = __shfl_sync(0xffffffffu, keys, w);
+        const unsigned first = base + __shfl_sync(0xffffffffu, inc - n, w);
+        sg.tiles = (sg.keys + kTile - 1) / kTile;
+        const int seg = (int)((begin - first) / sg.tiles);
+        sg.kvh = a.row_blocks == 1 ? seg : seg / a.row_blocks;
+        sg.rb = seg - sg.kvh * a.row_blocks;
+        tile = (int)(begin - first) - seg * sg.tiles;
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, inc, 31);
+    }
   }
   int left = (int)(end - begin);  // tiles of this CTA
 
@@ -247,37 +240,42 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
   float o[N64 * 4][NT][4];
   float F = 0.f;
   int keys_all = 0;                    // keys that every row keeps
+  bool fresh = true;                   // no key yet
 
-  auto begin_segment = [&](const Segment& c) {
-    const int kvh = c.kvh, rb = c.rb;
+  uint4 raw[NT][N64][sizeof(T)];       // the lane's 16 channels of each 64, as they come
+  auto load_rows = [&](const Segment& c) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = rb * ROWS + nt * 8 + g;
-      float x[N64][16];
-      if (row < a.rows) {
-        const int n = row_token(a, row);
-        const T* q = static_cast<const T*>(a.q) + (long long)c.b * a.qb + n * a.qn +
-                     (long long)(kvh * a.G + row - n * a.G) * a.qh + 16 * t;
+      const int row = c.rb * ROWS + nt * 8 + g;
+      const bool live = row < a.rows;
+      const int n = live ? row_token(a, row) : 0;
+      const T* q = static_cast<const T*>(a.q) + (long long)c.b * a.qb + n * a.qn +
+                   (long long)(c.kvh * a.G + (live ? row : 0) - n * a.G) * a.qh + 16 * t;
 #pragma unroll
-        for (int w = 0; w < N64; ++w) {
+      for (int w = 0; w < N64; ++w) {
+        raw[nt][w][0] = raw[nt][w][1] = make_uint4(0, 0, 0, 0);
+        if (live) {
           if (a.q_vec) {
-            uint4 r[2];
-            r[0] = *reinterpret_cast<const uint4*>(q + 64 * w);
-            r[1] = *reinterpret_cast<const uint4*>(q + 64 * w + 8);
-            const T* e = reinterpret_cast<const T*>(r);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[w][i] = to_f32<T>(e[i]);
+            raw[nt][w][0] = *reinterpret_cast<const uint4*>(q + 64 * w);
+            raw[nt][w][1] = *reinterpret_cast<const uint4*>(q + 64 * w + 8);
           } else {
+            T* e = reinterpret_cast<T*>(raw[nt][w]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[w][i] = to_f32<T>(q[64 * w + i]);
+            for (int i = 0; i < 16; ++i) e[i] = q[64 * w + i];
           }
         }
-      } else {
-#pragma unroll
-        for (int w = 0; w < N64; ++w)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[w][i] = 0.f;
       }
+    }
+  };
+  auto begin_segment = [&](const Segment& c) {
+    const int rb = c.rb;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float x[N64][16];
+#pragma unroll
+      for (int w = 0; w < N64; ++w)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[w][i] = to_f32<T>(reinterpret_cast<const T*>(raw[nt][w])[i]);
       // A power of two per row brings its largest value to 2^14 .. 2^15 in fp16: no
       // value down to 2^-28 of it becomes subnormal, and a sixteenth of it fits too.
       float top = 0.f;
@@ -324,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
         const int r = rb * ROWS + nt * 8 + 2 * t + c2;
         // rows that do not exist keep what the last token keeps
         lim[nt][c2] = r < a.rows ? max(0, c.keys - a.N + 1 + row_token(a, r)) : c.keys;
-        m[nt][c2] = kNoMax;
+        m[nt][c2] = 0.f;
         l[nt][c2] = 0.f;
 #pragma unroll
         for (int k = 0; k < NG; ++k) lo[nt][k][c2] = 0.f;
@@ -335,6 +333,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
         for (int k = 0; k < 4; ++k) o[i][nt][k] = 0.f;
     }
     F = __int_as_float(254 << 23);
+    fresh = true;
     keys_all = max(0, c.keys - a.N + 1);
   };
 
@@ -375,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
         for (int nt = 0; nt < NT; ++nt)
           mma16816(acc[NG == 2 ? w % N64 : 0][nt], a0, a1, a2, a3, qf[nt][w][s][0], qf[nt][w][s][1]);
       }
-    float sc[NT][4], sv[2][NG], lv[2][NG];
+    float x[NT][4], sv[2][NG], lv[2][NG];  // scores less the running maximum
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -388,12 +387,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int h = i >> 1, c2 = i & 1;
-        float u = scale_of(km[h][0]) * acc[0][nt][i], y = low_of(km[h][0]) * qs[nt][0][c2];
+        float u = scale_of(km[h][0]) * acc[0][nt][i], y = fmaf(low_of(km[h][0]), qs[nt][0][c2], -m[nt][c2]);
         if constexpr (NG == 2) {
           u = fmaf(scale_of(km[h][1]), acc[1][nt][i], u);
           y = fmaf(low_of(km[h][1]), qs[nt][1][c2], y);
         }
-        sc[nt][i] = fmaf(u, f[nt][c2], y);
+        x[nt][i] = fmaf(u, f[nt][c2], y);
       }
     const bool edge = key0 + 16 > keys_all;  // some row keeps only a part
     if (edge) {
@@ -404,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c2 = 0; c2 < 2; ++c2)
-            if (key >= lim[nt][c2]) sc[nt][2 * h + c2] = -INFINITY;
+            if (key >= lim[nt][c2]) x[nt][2 * h + c2] = -INFINITY;
         // past the sequence the page holds anything
         if (key >= keys)
 #pragma unroll
@@ -412,25 +411,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
       }
     }
     // raise the maxima, or lower F, where needed
-    float x[NT][4], svf[2][NG];
-    auto relative = [&] {
+    float svf[2][NG];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[nt][i] = sc[nt][i] - m[nt][i & 1];
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        svf[0][k] = sv[0][k] * F;
-        svf[1][k] = sv[1][k] * F;
-      }
-    };
-    relative();
+    for (int k = 0; k < NG; ++k) {
+      svf[0][k] = sv[0][k] * F;
+      svf[1][k] = sv[1][k] * F;
+    }
     float over = fmaxf(svf[0][0], svf[1][0]);
-    if constexpr (NG == 2) over = fmaxf(over, fmaxf(svf[0][1], svf[1][1]));
+    if constexpr (NG == 2) over = max3(over, svf[0][1], svf[1][1]);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      over = fmaxf(over, fmaxf(fmaxf(x[nt][0], x[nt][1]), fmaxf(x[nt][2], x[nt][3])));
-    if (__any_sync(0xffffffffu, over > 8.f)) {
+    for (int nt = 0; nt < NT; ++nt) over = max3(over, max3(x[nt][0], x[nt][1], x[nt][2]), x[nt][3]);
+    if (__any_sync(0xffffffffu, over > 8.f) || fresh) {
       float top = 0.f;
 #pragma unroll
       for (int k = 0; k < NG; ++k) top = fmaxf(top, fmaxf(sv[0][k], sv[1][k]));  // NaN is left aside
@@ -445,12 +436,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c2 = 0; c2 < 2; ++c2) {
-          float y = fmaxf(sc[nt][c2], sc[nt][2 + c2]);
+          float y = fmaxf(x[nt][c2], x[nt][2 + c2]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
-          const float to = fmaxf(m[nt][c2], y);
-          const float al = ex2(m[nt][c2] - to);
-          m[nt][c2] = to;
+          // the maximum's step; the first keys may set it below its start of 0
+          const float up = fresh ? (y > -INFINITY ? y : 0.f) : fmaxf(y, 0.f);
+          const float al = ex2(-up);
+          m[nt][c2] += up;
+          x[nt][c2] -= up;
+          x[nt][2 + c2] -= up;
           l[nt][c2] *= al;
 #pragma unroll
           for (int k = 0; k < NG; ++k) lo[nt][k][c2] *= al;
@@ -460,7 +454,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
             o[i][nt][2 + c2] *= al * ratio;
           }
         }
-      relative();
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        svf[0][k] = sv[0][k] * F;
+        svf[1][k] = sv[1][k] * F;
+      }
+      fresh = false;
     }
     // weights, and their products with the values' scales as the B operand
     // F is a power of two: 1/F by its exponent
@@ -540,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
   };
 
   // ---- merge the warps' results of a segment
-  auto end_segment = [&](const Segment& c, long long seg_begin) {
+  auto end_segment = [&](const Segment& c, bool cut_front, bool cut_back) {
     const int kvh = c.kvh, rb = c.rb;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -555,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
         if (wrong) l[nt][c2] = __int_as_float(0x7fffffff);  // no such page: the rows are undefined
         const int r = nt * 8 + 2 * t + c2;
         if (g == 0) {
-          s_m[warp * ROWS + r] = m[nt][c2];
+          s_m[warp * ROWS + r] = l[nt][c2] == 0.f ? kNoMax : m[nt][c2];
           s_l[warp * ROWS + r] = l[nt][c2];
         }
         const float down = 1.f / F;  // in range; 2^24 / F need not be
@@ -568,10 +567,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
         }
       }
     __syncthreads();
-    const bool whole = seg_begin >= begin && seg_begin + c.tiles <= end;
-    // the CTA's first cut segment goes to its slot 0 when it began before the CTA
-    const int slot = seg_begin < begin ? 0 : 1;
-    float* part = a.partials + (size_t)(2 * blockIdx.x + slot) * ROWS * (D + 2);
+    const bool whole = !cut_front && !cut_back;
+    // a CTA has at most two cut segments: one that began before it, one that goes on
+    float* part = a.partials + (size_t)(2 * blockIdx.x + (cut_front ? 0 : 1)) * ROWS * (D + 2);
     for (int e = threadIdx.x; e < ROWS * (D / 4); e += kThreads) {
       const int r = e / (D / 4), d = (e % (D / 4)) * 4;
       const int row = rb * ROWS + r;
@@ -613,9 +611,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
   };
 
   // ---- the segments of this CTA's part of the line
-  long long pos = begin;
   while (true) {
-    const long long seg_begin = pos - tile;
+    const int start = tile;
     const int stop = min(sg.tiles, tile + left);
     {
       const size_t head = (size_t)sg.kvh * a.page_size;
@@ -626,8 +623,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
     }
     wrong = false;
     left -= stop - tile;
-    pos += stop - tile;
     lookup(tile);
+    load_rows(sg);
     load(tile, 0);
     if (tile + 1 < stop) lookup(tile + 1);
     begin_segment(sg);
@@ -648,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
       stage ^= 1;
     }
     if (wrong && lane == 0) atomicOr(a.status, DEV_BAD_INDEX);
-    end_segment(sg, seg_begin);
+    end_segment(sg, start > 0, stop < sg.tiles);
     if (left == 0) break;
     // the next segment that has tiles
     tile = 0;
@@ -674,7 +671,6 @@ constexpr int kJoinMax = 1024;  // parts whose weights are kept; a segment has a
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kJoin) kv_attn_join_kernel(const __grid_constant__ AttnArgs a, int grid) {
   constexpr int LANES = D / 4, LINES = kJoin / LANES;
-  __shared__ Pair s_sum[kJoin / 32];
   __shared__ float s_w[kJoinMax], s_top[kJoin / 32], s_total[kJoin / 32];
   __shared__ float4 s_v[LINES][LANES];
   const int per_seq = a.H * a.rows;
@@ -694,18 +690,11 @@ __global__ void __launch_bounds__(kJoin) kv_attn_join_kernel(const __grid_consta
     for (int d = threadIdx.x; d < D; d += kJoin) out[d] = from_f32<T>(wrong ? __int_as_float(0x7fffffff) : 0.f);
     return;
   }
-  long long mine_before = 0, mine = 0;
-  for (int i = threadIdx.x; i < a.B; i += kJoin) {
-    const int k = tiles_of(a, i);
-    mine += k;
-    if (i < b) mine_before += k;
-  }
-  const Pair s = block_sum<kJoin / 32>(mine, mine_before, s_sum);
+  unsigned before;
+  const Line line(count_tiles(a, b, &before) * segs, grid);
+  before = before * segs + (unsigned)seg * tiles;
+  const int c0 = (int)line.owner(before), c1 = (int)line.owner(before + tiles - 1);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const long long total = s.a * segs, before = s.b * segs + (long long)seg * tiles;
-  const long long ctas = total < grid ? total : grid;
-  // CTA c holds tiles [c * total / ctas, (c + 1) * total / ctas)
-  const int c0 = (int)(((before + 1) * ctas - 1) / total), c1 = (int)(((before + tiles) * ctas - 1) / total);
   if (c0 == c1) return;  // whole in one CTA, which wrote it
   const int parts = c1 - c0 + 1;
   // the first CTA's part began in it (slot 1), the others' began before them (slot 0)
@@ -731,10 +720,10 @@ __global__ void __launch_bounds__(kJoin) kv_attn_join_kernel(const __grid_consta
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_total[warp] = sum;
   __syncthreads();
-  const int col = threadIdx.x % LANES, line = threadIdx.x / LANES;
+  const int col = threadIdx.x % LANES, first = threadIdx.x / LANES;
   float4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int i = line; i < parts; i += LINES) {
+  for (int i = first; i < parts; i += LINES) {
     const float4 y = *reinterpret_cast<const float4*>(part(i) + r * D + 4 * col);
     const float w = s_w[i];
     v.x = fmaf(w, y.x, v.x);
@@ -742,9 +731,9 @@ __global__ void __launch_bounds__(kJoin) kv_attn_join_kernel(const __grid_consta
     v.z = fmaf(w, y.z, v.z);
     v.w = fmaf(w, y.w, v.w);
   }
-  s_v[line][col] = v;
+  s_v[first][col] = v;
   __syncthreads();
-  if (line == 0) {
+  if (first == 0) {
     float all = 0.f;
 #pragma unroll
     for (int w = 0; w < kJoin / 32; ++w) all += s_total[w];
@@ -773,9 +762,9 @@ int launch(AttnArgs& a, cudaStream_t st) {
   constexpr int ROWS = 8 * NT;
   constexpr size_t smem = (size_t)kWarps * kStages * kSteps * R::kStage + (size_t)kWarps * ROWS * (D + 6) * sizeof(float);
   a.row_blocks = (a.rows + ROWS - 1) / ROWS;
-  const long long segs = (long long)a.B * a.H * a.row_blocks;
-  if (segs >= (1LL << 31)) {
-    set_error("b2_kv_cache_attn: B * H * row blocks must be < 2^31");
+  const double tiles = (double)a.B * a.H * a.row_blocks * (((double)a.max_pages * a.page_size + kTile) / kTile);
+  if (tiles >= 2147483648.0) {
+    set_error("b2_kv_cache_attn: B * H * row blocks * (max_pages * page_size / %d) must be < 2^31", kTile);
     return B2_EINVAL;
   }
   auto kern = kv_attn_kernel<T, D, GROUP, NT>;
