@@ -18,11 +18,16 @@
 //
 // Bound: HBM. One thread owns one word of keys and the same word of values; a
 // group's extremes take 3 or 4 shuffles.
+#include <type_traits>
+
 #include "b2_common.cuh"
 #include "decoder.cuh"
+#include "fa_math.cuh"
 
 namespace b2 {
 namespace {
+
+using namespace fa;
 
 __device__ uint32_t g_kv_cache_status;
 
@@ -54,50 +59,74 @@ struct RowsArgs {
   int slots64;
 };
 
-// 8 values of one row
+// 8 values of one row, as they come
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+__device__ __forceinline__ void load8(const T* p, T (&x)[8]) {
   if constexpr (VEC) {
-    uint4 r[sizeof(T) / 2];
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
-    const T* e = reinterpret_cast<const T*>(r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(e[i]);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(p)[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(p[i]);
+    for (int i = 0; i < 8; ++i) x[i] = p[i];
   }
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+__device__ __forceinline__ void store8(T* p, const T (&x)[8]) {
   if constexpr (VEC) {
-    uint4 r[sizeof(T) / 2];
-    T* e = reinterpret_cast<T*>(r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(f[i]);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(x)[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = from_f32<T>(f[i]);
+    for (int i = 0; i < 8; ++i) p[i] = x[i];
+  }
+}
+
+__device__ __forceinline__ __nv_bfloat162 max2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2_nan(a, b); }
+__device__ __forceinline__ __half2 max2(__half2 a, __half2 b) { return __hmax2_nan(a, b); }
+
+__device__ __forceinline__ __nv_bfloat162 low_pair(__nv_bfloat162 a, __nv_bfloat162 b) { return __lows2bfloat162(a, b); }
+__device__ __forceinline__ __half2 low_pair(__half2 a, __half2 b) { return __lows2half2(a, b); }
+__device__ __forceinline__ __nv_bfloat162 high_pair(__nv_bfloat162 a, __nv_bfloat162 b) { return __highs2bfloat162(a, b); }
+__device__ __forceinline__ __half2 high_pair(__half2 a, __half2 b) { return __highs2half2(a, b); }
+
+// Largest and lowest value of a group of LANES * 8 values; NaN when it holds one.
+// 16-bit types: compared two at a time in their own type, (max, -min) in one word, so
+// that one shuffle and one packed maximum serve both (every step is exact).
+template <int LANES, typename T>
+__device__ __forceinline__ void extremes(const T (&x)[8], float& hi, float& lo) {
+  if constexpr (sizeof(T) == 2) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* p = reinterpret_cast<const T2*>(x);
+    T2 up = max2(max2(p[0], p[1]), max2(p[2], p[3]));
+    T2 dn = max2(max2(__hneg2(p[0]), __hneg2(p[1])), max2(__hneg2(p[2]), __hneg2(p[3])));
+    T2 m = max2(low_pair(up, dn), high_pair(up, dn));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      const uint32_t y = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<uint32_t*>(&m), o);
+      m = max2(m, *reinterpret_cast<const T2*>(&y));
+    }
+    hi = to_f32<T>(m.x);
+    lo = -to_f32<T>(m.y);
+  } else {
+    hi = lo = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      hi = max_nan(hi, x[i]);
+      lo = fminf(lo, x[i]);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    }
   }
 }
 
 // The code word of 8 values and the group's (scale, lo) as two packed bf16.
-template <int LANES>
-__device__ __forceinline__ uint32_t quantise(const float (&x)[8], uint32_t& meta) {
-  float hi = x[0], lo = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    hi = max_nan(hi, x[i]);
-    lo = fminf(lo, x[i]);
-  }
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) {
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-  }
+template <int LANES, typename T>
+__device__ __forceinline__ uint32_t quantise(const T (&x)[8], uint32_t& meta) {
+  float hi, lo;
+  extremes<LANES>(x, hi, lo);
   const float low = bf16_down(lo);
   const float step = (hi - low) * (1.0f / 15.0f);
   const float scale = bf16_up(step);
@@ -108,15 +137,21 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[8], uint32_t& meta
   meta = (__float_as_uint(scale) >> 16) | (__float_as_uint(low) & 0xffff0000u);
   // below 2^-126 the reciprocal may overflow; the group reads back as lo then
   const float inv = scale >= 1.17549435e-38f ? 1.0f / scale : 0.0f;
-  // adding 1.5 * 2^23 rounds to the nearest integer (ties to even) and leaves it
-  // in the low bits; the constant's own bits add up to the number subtracted.
-  uint32_t word = 0;
+  // (x - low) * inv is at most 15 (1 + 2^-21), scale being rounded up. Adding
+  // 1.5 * 2^23 rounds it to the nearest integer (ties to even) and leaves that in
+  // the low bits; what the constant's own bits add to the word is subtracted.
+  constexpr uint32_t kMagic = 0x4b400000u;
+  uint32_t word = 0, bias = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = fminf((x[i] - low) * inv, 15.0f) + 12582912.0f;
-    word += (__float_as_uint(t) & 15u) << (4 * i);
+  for (int i = 0; i < 8; i += 2) {
+    f2_t y = f2_add(f2_pack(to_f32<T>(x[i]), to_f32<T>(x[i + 1])), f2_pack(-low, -low));
+    y = f2_add(f2_mul(y, f2_pack(inv, inv)), f2_pack(12582912.0f, 12582912.0f));
+    float y0, y1;
+    f2_unpack(y, y0, y1);
+    word += (__float_as_uint(y0) << (4 * i)) + (__float_as_uint(y1) << (4 * i + 4));
+    bias += (kMagic << (4 * i)) + (kMagic << (4 * i + 4));
   }
-  return word;
+  return word - bias;
 }
 
 template <int D>
@@ -133,7 +168,7 @@ __global__ void __launch_bounds__(kCacheThreads) kv_write_kernel(const __grid_co
   // threads past the last row repeat it without storing: the shuffles need them
   const unsigned r = row < a.rows ? row : a.rows - 1;
   const unsigned token = r / a.H, head = r - token * a.H;
-  float k[8], v[8];
+  __align__(16) T k[8], v[8];
   load8<T, VEC>(static_cast<const T*>(a.k) + (long long)token * a.kt + (long long)head * a.kh + lane * 8, k);
   load8<T, VEC>(static_cast<const T*>(a.v) + (long long)token * a.vt + (long long)head * a.vh + lane * 8, v);
   const long long slot = a.slots64 ? static_cast<const long long*>(a.slots)[token]
@@ -155,13 +190,19 @@ __global__ void __launch_bounds__(kCacheThreads) kv_write_kernel(const __grid_co
   }
 }
 
-__device__ __forceinline__ void values8(uint32_t word, uint32_t meta, float (&f)[8]) {
+template <typename T>
+__device__ __forceinline__ void values8(uint32_t word, uint32_t meta, T (&x)[8]) {
   const float s = __uint_as_float(meta << 16), lo = __uint_as_float(meta & 0xffff0000u);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 8; i += 2) {
     // 2^23 + c minus 2^23 is the code as a float
-    const float c = __uint_as_float(0x4b000000u | ((word >> (4 * i)) & 15u)) - 8388608.0f;
-    f[i] = fmaf(c, s, lo);
+    f2_t y = f2_pack(__uint_as_float(0x4b000000u | ((word >> (4 * i)) & 15u)),
+                     __uint_as_float(0x4b000000u | ((word >> (4 * i + 4)) & 15u)));
+    y = f2_fma(f2_add(y, f2_pack(-8388608.0f, -8388608.0f)), f2_pack(s, s), f2_pack(lo, lo));
+    float y0, y1;
+    f2_unpack(y, y0, y1);
+    x[i] = from_f32<T>(y0);
+    x[i + 1] = from_f32<T>(y1);
   }
 }
 
@@ -175,7 +216,7 @@ __global__ void __launch_bounds__(kCacheThreads) kv_read_kernel(const __grid_con
   const unsigned token = row / a.H, head = row - token * a.H;
   const long long slot = a.slots64 ? static_cast<const long long*>(a.slots)[token]
                                    : static_cast<const int*>(a.slots)[token];
-  float k[8], v[8];
+  __align__(16) T k[8], v[8];
   if (slot >= 0 && slot < (long long)a.capacity) {
     const unsigned page = (unsigned)slot / a.page_size, place = (unsigned)slot - page * a.page_size;
     const size_t at = ((size_t)page * a.H + head) * a.page_size + place;
@@ -190,7 +231,7 @@ __global__ void __launch_bounds__(kCacheThreads) kv_read_kernel(const __grid_con
     const float fill = slot < 0 ? 0.f : __int_as_float(0x7fffffff);
     if (slot >= 0 && lane == 0) atomicOr(&g_kv_cache_status, DEV_BAD_INDEX);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) k[i] = v[i] = fill;
+    for (int i = 0; i < 8; ++i) k[i] = v[i] = from_f32<T>(fill);
   }
   store8<T, VEC>(static_cast<T*>(a.k) + (long long)token * a.kt + (long long)head * a.kh + lane * 8, k);
   store8<T, VEC>(static_cast<T*>(a.v) + (long long)token * a.vt + (long long)head * a.vh + lane * 8, v);

@@ -7,27 +7,41 @@
 //
 // Bound: HBM. Each value is read once and written once; the table row of a
 // token (4R bytes) is shared by its heads and mostly served by the L1 cache.
-// A lane group owns HPT heads of one token: each lane holds the two vectors
+// A lane group owns four heads of one token: each lane holds the two vectors
 // whose channels rotate into one another, so the rotation needs no exchange,
 // and the norm one shuffle tree; the lane's table values are loaded once for
-// all HPT heads, whose loads are issued together before any arithmetic.
+// all four heads, whose loads are issued together before any arithmetic.
+// 16-bit inputs are bound by instructions as much as by HBM (converting, norm and
+// rotation take about ten a value): vectors of 4 channels, 16 lanes a head of 128,
+// leave registers for 24 warps per SM; with vectors of 8, 16 warps, it took 92 us
+// where it takes 81 now (16384 tokens, 32 + 8 heads of 128, bf16: 4.2 TB/s; fp32
+// 104 us, 6.5 TB/s).
 // The arithmetic is fp32 throughout; only the result is rounded to x's type.
+#include <type_traits>
+
 #include "b2_common.cuh"
 #include "decoder.cuh"
+#include "fa_math.cuh"
 
 namespace b2 {
 namespace {
 
+using namespace fa;
+
 __device__ uint32_t g_rope_status;
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeMaxDim = 512;
 
 template <int BYTES> struct RawVec;
 template <> struct RawVec<16> { using type = uint4; };
 template <> struct RawVec<8> { using type = uint2; };
 template <> struct RawVec<4> { using type = uint32_t; };
 template <> struct RawVec<2> { using type = uint16_t; };
+
+// Heads per lane group, and CTAs per SM below: measured on 16384 tokens of 32 + 8
+// heads of 128, bf16 with norm, 4 heads and 3 CTAs (80 registers) 81 us; 2 heads and
+// 4 CTAs 91; 2 and 5 83; 4 and 4 (64 registers, spills) 110.
+constexpr int kHeads = 4;
 
 struct RopeTensor {
   const void* x;
@@ -46,14 +60,60 @@ struct RopeArgs {
   unsigned items_q;      // of these, the queries'
   unsigned total;        // items * tokens
   int pos64, D, R, log_tpr, heads_per_group;
-  float eps;
+  float eps, inv_dim;
 };
+
+// VE values, two to a packed fp32 pair where VE is even.
+template <int VE>
+struct Vals {
+  static constexpr bool kPacked = VE % 2 == 0;
+  static constexpr int N = kPacked ? VE / 2 : VE;
+  using E = typename std::conditional<kPacked, f2_t, float>::type;
+  E v[N];
+  __device__ __forceinline__ Vals() {}
+  __device__ __forceinline__ explicit Vals(const float (&x)[VE]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if constexpr (kPacked) v[i] = f2_pack(x[2 * i], x[2 * i + 1]);
+      else v[i] = x[i];
+  }
+  __device__ __forceinline__ void fill(float x) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if constexpr (kPacked) v[i] = f2_pack(x, x);
+      else v[i] = x;
+  }
+  __device__ __forceinline__ void get(float (&x)[VE]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if constexpr (kPacked) f2_unpack(v[i], x[2 * i], x[2 * i + 1]);
+      else x[i] = v[i];
+  }
+};
+template <int VE>
+__device__ __forceinline__ Vals<VE> mul(const Vals<VE>& a, const Vals<VE>& b) {
+  Vals<VE> r;
+#pragma unroll
+  for (int i = 0; i < Vals<VE>::N; ++i)
+    if constexpr (Vals<VE>::kPacked) r.v[i] = f2_mul(a.v[i], b.v[i]);
+    else r.v[i] = a.v[i] * b.v[i];
+  return r;
+}
+template <int VE>
+__device__ __forceinline__ Vals<VE> fma(const Vals<VE>& a, const Vals<VE>& b, const Vals<VE>& c) {
+  Vals<VE> r;
+#pragma unroll
+  for (int i = 0; i < Vals<VE>::N; ++i)
+    if constexpr (Vals<VE>::kPacked) r.v[i] = f2_fma(a.v[i], b.v[i], c.v[i]);
+    else r.v[i] = fmaf(a.v[i], b.v[i], c.v[i]);
+  return r;
+}
 
 // One lane holds NP units of 2*VE values of each head. Unit u < R/(2 VE) is
 // rotated: channels [u VE, u VE + VE) with those R/2 above (half layout), or the
 // 2 VE neighbours from 2 u VE (interleaved). The other units are copied.
-template <typename T, int VE, int NP, int HPT, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
+template <typename T, int VE, int NP, bool INTER>
+__global__ void __launch_bounds__(kRopeThreads, 3) rope_kernel(const __grid_constant__ RopeArgs a) {
   using Raw = typename RawVec<VE * (int)sizeof(T)>::type;
   const int tpr = 1 << a.log_tpr;
   const unsigned gid = (blockIdx.x * kRopeThreads + threadIdx.x) >> a.log_tpr;
@@ -68,24 +128,29 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
   const int nh = live ? min(a.heads_per_group, in.heads - h0) : 0;
   const T* x = static_cast<const T*>(in.x) + (long long)token * in.xt + (long long)h0 * in.xh;
   T* y = static_cast<T*>(in.y) + (long long)token * in.yt + (long long)h0 * in.yh;
+  // between a group's heads; the host keeps this within 32 bits
+  const int xh = (int)in.xh, yh = (int)in.yh;
   const T* w = static_cast<const T*>(in.w);
   const int units = a.D / (2 * VE), turned = a.R / (2 * VE);
 
   auto first = [&](int u) { return INTER || u >= turned ? 2 * u * VE : u * VE; };
   auto second = [&](int u) { return INTER || u >= turned ? 2 * u * VE + VE : u * VE + a.R / 2; };
 
-  Raw raw[HPT][NP][2];
+  Raw raw[kHeads][NP][2];
 #pragma unroll
-  for (int i = 0; i < HPT; ++i)
+  for (int p = 0; p < NP; ++p) {
+    const int u = lane + p * tpr;
+    const T* const x0 = x + first(u);
+    const int gap = second(u) - first(u);
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const int u = lane + p * tpr;
+    for (int i = 0; i < kHeads; ++i) {
       raw[i][p][0] = raw[i][p][1] = Raw{};
       if (i < nh && u < units) {
-        raw[i][p][0] = *reinterpret_cast<const Raw*>(x + i * in.xh + first(u));
-        raw[i][p][1] = *reinterpret_cast<const Raw*>(x + i * in.xh + second(u));
+        raw[i][p][0] = *reinterpret_cast<const Raw*>(x0 + i * xh);
+        raw[i][p][1] = *reinterpret_cast<const Raw*>(x0 + i * xh + gap);
       }
     }
+  }
 
   long long pos = 0;
   if (live) pos = a.pos64 ? static_cast<const long long*>(a.positions)[token]
@@ -95,133 +160,169 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
   const bool in_table = pos >= 0 && pos < a.P;
   if (live && !in_table && lane == 0) atomicOr(&g_rope_status, DEV_BAD_INDEX);
   const float* row = a.table + (in_table ? pos : 0) * a.R;
-  float cs[NP][VE], sn[NP][VE];
+  // Per lane and token, for all of its heads: with the weight w folded into the
+  // angles, a' = r (a c w_a - b s w_b) and b' = r (b c w_b + a s w_a), r the head's
+  // 1/rms: six operations a pair in place of eight, and four heads share these.
+  float ca[NP][VE], sb[NP][VE], cb[NP][VE], sa[NP][VE];
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
     const int u = lane + p * tpr;
+    float wa[VE], wb[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
-      cs[p][e] = 1.f;
-      sn[p][e] = 0.f;
+      ca[p][e] = cb[p][e] = wa[e] = wb[e] = 1.f;
+      sa[p][e] = sb[p][e] = 0.f;
     }
     if (live && u < turned) {
+      float cs[VE], sn[VE];
       if (in_table) {
         if constexpr (VE >= 4) {
 #pragma unroll
           for (int e = 0; e < VE; e += 4) {
-            *reinterpret_cast<float4*>(&cs[p][e]) = __ldg(reinterpret_cast<const float4*>(row + u * VE + e));
-            *reinterpret_cast<float4*>(&sn[p][e]) = __ldg(reinterpret_cast<const float4*>(row + a.R / 2 + u * VE + e));
+            *reinterpret_cast<float4*>(&cs[e]) = __ldg(reinterpret_cast<const float4*>(row + u * VE + e));
+            *reinterpret_cast<float4*>(&sn[e]) = __ldg(reinterpret_cast<const float4*>(row + a.R / 2 + u * VE + e));
           }
         } else {
 #pragma unroll
           for (int e = 0; e < VE; ++e) {
-            cs[p][e] = __ldg(row + u * VE + e);
-            sn[p][e] = __ldg(row + a.R / 2 + u * VE + e);
+            cs[e] = __ldg(row + u * VE + e);
+            sn[e] = __ldg(row + a.R / 2 + u * VE + e);
           }
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) cs[p][e] = sn[p][e] = __int_as_float(0x7fffffff);
+        for (int e = 0; e < VE; ++e) cs[e] = sn[e] = __int_as_float(0x7fffffff);
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        ca[p][e] = cb[p][e] = cs[e];
+        sa[p][e] = sn[e];
+        sb[p][e] = -sn[e];
+      }
+    }
+    if (w && live && u < units) {
+      const Raw wr[2] = {__ldg(reinterpret_cast<const Raw*>(w + first(u))), __ldg(reinterpret_cast<const Raw*>(w + second(u)))};
+      const T* e0 = reinterpret_cast<const T*>(wr);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        wa[e] = to_f32<T>(e0[INTER ? 2 * e : e]);
+        wb[e] = to_f32<T>(e0[INTER ? 2 * e + 1 : VE + e]);
+        ca[p][e] *= wa[e];
+        sa[p][e] *= wa[e];
+        cb[p][e] *= wb[e];
+        sb[p][e] *= wb[e];
       }
     }
   }
 
+  // the pairs' first and second values, each head's
+  float va[kHeads][NP][VE], vb[kHeads][NP][VE];
 #pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    float v[NP][2 * VE];
-    float ss = 0.f;
-#pragma unroll
-    for (int p = 0; p < NP; ++p)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const T* e = reinterpret_cast<const T*>(&raw[i][p][c]);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          v[p][c * VE + j] = to_f32<T>(e[j]);
-          ss = fmaf(v[p][c * VE + j], v[p][c * VE + j], ss);
-        }
-      }
-    if (w) {  // uniform in the lane group
-      // lanes of other groups may take the other branch: a group's shuffles
-      // name its own lanes only
-      const unsigned mask = tpr == 32 ? 0xffffffffu : ((1u << tpr) - 1u) << (threadIdx.x & 31 & ~(tpr - 1));
-      for (int o = tpr >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-      const float r = rsqrtf(ss / (float)a.D + a.eps);
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        const int u = lane + p * tpr;
-        if (u < units) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const Raw wr = __ldg(reinterpret_cast<const Raw*>(w + (c ? second(u) : first(u))));
-            const T* e = reinterpret_cast<const T*>(&wr);
-#pragma unroll
-            for (int j = 0; j < VE; ++j) v[p][c * VE + j] *= r * to_f32<T>(e[j]);
-          }
-        }
-      }
-    }
+  for (int i = 0; i < kHeads; ++i)
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const int u = lane + p * tpr;
-      // units that are not rotated have c = 1, s = 0 but are left alone: 0 * inf
-      if (u < turned) {
+      const T* x0 = reinterpret_cast<const T*>(raw[i][p]);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          float& lo = v[p][INTER ? 2 * e : e];
-          float& hi = v[p][INTER ? 2 * e + 1 : VE + e];
-          const float t = lo * cs[p][e] - hi * sn[p][e];
-          hi = hi * cs[p][e] + lo * sn[p][e];
-          lo = t;
-        }
+      for (int e = 0; e < VE; ++e) {
+        va[i][p][e] = to_f32<T>(x0[INTER ? 2 * e : e]);
+        vb[i][p][e] = to_f32<T>(x0[INTER ? 2 * e + 1 : VE + e]);
       }
-      if (i < nh && u < units) {
-        Raw out[2];
+    }
+  // 1/rms of each head; the heads' shuffle trees run beside one another
+  float r[kHeads];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          T* e = reinterpret_cast<T*>(&out[c]);
+  for (int i = 0; i < kHeads; ++i) r[i] = 1.f;
+  if (a.in[0].w || a.in[1].w) {  // the whole grid alike, so every lane takes part
 #pragma unroll
-          for (int j = 0; j < VE; ++j) e[j] = from_f32<T>(v[p][c * VE + j]);
-        }
-        *reinterpret_cast<Raw*>(y + i * in.yh + first(u)) = out[0];
-        *reinterpret_cast<Raw*>(y + i * in.yh + second(u)) = out[1];
+    for (int i = 0; i < kHeads; ++i) {
+      Vals<VE> s2;
+      s2.fill(0.f);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const Vals<VE> ya(va[i][p]), yb(vb[i][p]);
+        s2 = fma(ya, ya, s2);
+        s2 = fma(yb, yb, s2);
       }
+      float t[VE];
+      s2.get(t);
+      r[i] = t[0];
+#pragma unroll
+      for (int e = 1; e < VE; ++e) r[i] += t[e];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      if (o < tpr)
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) r[i] += __shfl_xor_sync(0xffffffffu, r[i], o);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) r[i] = w ? rsqrtf(fmaf(r[i], a.inv_dim, a.eps)) : 1.f;
+  }
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    const int u = lane + p * tpr;
+    const Vals<VE> kca(ca[p]), ksb(sb[p]), kcb(cb[p]), ksa(sa[p]);
+    T* const y0 = y + first(u);
+    const int gap = second(u) - first(u);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      if (!(i < nh && u < units)) continue;
+      const Vals<VE> xa(va[i][p]), xb(vb[i][p]);
+      Vals<VE> scale;
+      scale.fill(r[i]);
+      Vals<VE> ya = mul(xa, kca), yb = mul(xb, kcb);
+      if (u < turned) {  // the others only take the norm: 0 * inf is not 0
+        ya = fma(xb, ksb, ya);
+        yb = fma(xa, ksa, yb);
+      }
+      float oa[VE], ob[VE];
+      mul(ya, scale).get(oa);
+      mul(yb, scale).get(ob);
+      Raw out[2];
+      T* e0 = reinterpret_cast<T*>(out);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        e0[INTER ? 2 * e : e] = from_f32<T>(oa[e]);
+        e0[INTER ? 2 * e + 1 : VE + e] = from_f32<T>(ob[e]);
+      }
+      *reinterpret_cast<Raw*>(y0 + i * yh) = out[0];
+      *reinterpret_cast<Raw*>(y0 + i * yh + gap) = out[1];
     }
   }
 }
 
-template <typename T, int VE, int HPT>
+template <typename T, int VE, int NP>
 int launch(RopeArgs& a, long long tokens, bool inter, cudaStream_t st) {
-  constexpr int NP = kRopeMaxDim / (2 * VE * 32) > 0 ? kRopeMaxDim / (2 * VE * 32) : 1;
+  // Heads further apart than 32 bits allow go to a group each.
+  const long long far = 1LL << 28;
+  const bool near = a.in[0].xh < far && a.in[0].yh < far && a.in[1].xh < far && a.in[1].yh < far &&
+                    a.in[0].xh > -far && a.in[0].yh > -far && a.in[1].xh > -far && a.in[1].yh > -far;
+  const int per = near ? kHeads : 1;
   const int units = a.D / (2 * VE);
   a.log_tpr = 0;
   while ((1 << a.log_tpr) < units && a.log_tpr < 5) ++a.log_tpr;
-  a.heads_per_group = HPT;
-  a.items_q = (unsigned)((a.in[0].heads + HPT - 1) / HPT);
-  a.items = a.items_q + (unsigned)((a.in[1].heads + HPT - 1) / HPT);
+  a.heads_per_group = per;
+  a.items_q = (unsigned)((a.in[0].heads + per - 1) / per);
+  a.items = a.items_q + (unsigned)((a.in[1].heads + per - 1) / per);
   const long long total = tokens * a.items;
   const long long threads = total << a.log_tpr;
-  if (threads + kRopeThreads >= (1LL << 31)) {
+  if (threads + kRopeThreads >= (1LL << 32)) {
     set_error("b2_qk_norm_rope: %lld tokens x %u lane groups are too many for one launch", tokens, a.items);
     return B2_EINVAL;
   }
   a.total = (unsigned)total;
   const unsigned grid = (unsigned)((threads + kRopeThreads - 1) / kRopeThreads);
-  if (inter) rope_kernel<T, VE, NP, HPT, true><<<grid, kRopeThreads, 0, st>>>(a);
-  else rope_kernel<T, VE, NP, HPT, false><<<grid, kRopeThreads, 0, st>>>(a);
+  if (inter) rope_kernel<T, VE, NP, true><<<grid, kRopeThreads, 0, st>>>(a);
+  else rope_kernel<T, VE, NP, false><<<grid, kRopeThreads, 0, st>>>(a);
   B2_CHECK_LAUNCH();
   return B2_OK;
 }
 
+// A head of up to 64 VE channels is one unit a lane; the longest take several.
 template <typename T>
 int launch_typed(RopeArgs& a, long long tokens, bool inter, int ve, cudaStream_t st) {
-  constexpr int HPT = sizeof(T) == 2 ? 4 : 2;
-  if constexpr (sizeof(T) == 2) {
-    if (ve >= 8) return launch<T, 8, HPT>(a, tokens, inter, st);
-  }
-  if (ve >= 4) return launch<T, 4, HPT>(a, tokens, inter, st);
-  if (ve >= 2) return launch<T, 2, HPT>(a, tokens, inter, st);
-  return launch<T, 1, HPT>(a, tokens, inter, st);
+  if (ve == 4) return a.D <= 256 ? launch<T, 4, 1>(a, tokens, inter, st) : launch<T, 4, 2>(a, tokens, inter, st);
+  if (ve == 2) return a.D <= 128 ? launch<T, 2, 1>(a, tokens, inter, st) : launch<T, 2, 4>(a, tokens, inter, st);
+  return a.D <= 128 ? launch<T, 1, 2>(a, tokens, inter, st) : launch<T, 1, 8>(a, tokens, inter, st);
 }
 
 }  // namespace
@@ -238,10 +339,11 @@ int rope_launch(const RopeCall& c, cudaStream_t st) {
   a.D = (int)c.D;
   a.R = (int)c.R;
   a.eps = c.eps;
-  // Widest vector that divides the rotated half, the row and every stride and
-  // pointer (16 bytes at most).
+  a.inv_dim = 1.0f / (float)c.D;
+  // Widest vector, up to four values, that divides the rotated half, the row and
+  // every stride and pointer.
   const int es = dtype_size(c.dtype);
-  int ve = 16 / es;
+  int ve = 4;
   auto fits = [&](int v) {
     if ((c.R / 2) % v || c.D % (2 * v)) return false;
     if (v >= 4 && (reinterpret_cast<uintptr_t>(c.table) & 15)) return false;
