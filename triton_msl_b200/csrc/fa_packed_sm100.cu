@@ -23,7 +23,7 @@
 //  * V rows of later tokens of the same sequence (causal) cannot be zeroed, as
 //    later queries of the tile use them. A result row that is not finite is
 //    looked at again: if a masked key of its last blocks is not finite, the row
-//    is computed anew over its own keys (fix_row).
+//    is computed anew over its own keys, at the end.
 //  * NaN scores make the row NaN: the running maximum propagates NaN, since the
 //    polynomial exponential would not.
 // D <= 64 runs on 64-channel tiles, D <= 128 on 128; TMA fills the channels
@@ -63,8 +63,7 @@ struct __align__(16) Entry {
 };
 static_assert(sizeof(Entry) == 32, "two 16-byte loads");
 constexpr int kPlanHeader = 64;      // bytes before the entries: the number of them
-constexpr int kPlanClasses = 2048;   // key-block counts told apart by the sort
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanClasses = 256;    // key-block counts told apart by the sort
 
 struct PlanArgs {
   const int32_t *cu_q, *cu_k;
@@ -92,14 +91,19 @@ __device__ __forceinline__ Entry make_entry(const PlanArgs& a, const packed::Spa
   return e;
 }
 
+// Counts up to 127 have a class each, above that 32 share one.
+__device__ __forceinline__ int plan_class(int blocks) {
+  return kPlanClasses - 1 - (blocks < 128 ? blocks : min(128 + ((blocks - 128) >> 5), kPlanClasses - 1));
+}
+
 // One CTA: a counting sort of the entries by key blocks, most first. The order
 // within a class is the atomics' and changes nothing but the schedule.
-__global__ void __launch_bounds__(kPlanThreads) fa_packed_plan_kernel(const PlanArgs a) {
+__global__ void __launch_bounds__(1024) fa_packed_plan_kernel(const PlanArgs a) {
   __shared__ int hist[kPlanClasses];
-  __shared__ int part[kPlanThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kPlanThreads / 32;
+  __shared__ int part[kPlanClasses / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   asm volatile("griddepcontrol.launch_dependents;");
-  for (int i = threadIdx.x; i < kPlanClasses; i += kPlanThreads) hist[i] = 0;
+  if (threadIdx.x < kPlanClasses) hist[threadIdx.x] = 0;
   __syncthreads();
   auto for_entries = [&](auto&& f) {
     for (int b = warp - 1; b <= a.B; b += warps) {
@@ -107,30 +111,31 @@ __global__ void __launch_bounds__(kPlanThreads) fa_packed_plan_kernel(const Plan
       const packed::Span k = b < 0 || b >= a.B ? packed::Span{0, 0} : packed::span_of(a.cu_k, b, a.B, a.Tk);
       for (int blk = lane; blk * 2 * a.R < q.len; blk += 32) {
         const Entry e = make_entry(a, q, k, blk);
-        f(e, kPlanClasses - 1 - min(max(e.n0, e.n1), kPlanClasses - 1));
+        f(e, plan_class(max(e.n0, e.n1)));
       }
     }
   };
   for_entries([&](const Entry&, int cls) { atomicAdd(&hist[cls], 1); });
-  for (int b = threadIdx.x; b < a.B; b += kPlanThreads)
+  for (int b = threadIdx.x; b < a.B; b += blockDim.x)
     if (packed::span_bad(a.cu_q, b, a.Tq) || packed::span_bad(a.cu_k, b, a.Tk))
       atomicOr(&g_packed_status, DEV_BAD_INDEX);
   __syncthreads();
-  // exclusive prefix sums of the classes, two per thread
-  const int h0 = hist[2 * threadIdx.x], h1 = hist[2 * threadIdx.x + 1];
-  int inc = h0 + h1;
+  // prefix sums of the classes, one per thread of the first eight warps
+  int own = 0, inc = 0;
+  if (threadIdx.x < kPlanClasses) {
+    own = inc = hist[threadIdx.x];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += up;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) part[warp] = inc;
   }
-  if (lane == 31) part[warp] = inc;
   __syncthreads();
-  int before = 0;
-  for (int w = 0; w < warp; ++w) before += part[w];
-  const int ex = before + inc - h0 - h1;
-  hist[2 * threadIdx.x] = ex;
-  hist[2 * threadIdx.x + 1] = ex + h0;
+  if (threadIdx.x < kPlanClasses) {
+    for (int w = 0; w < warp; ++w) inc += part[w];
+    hist[threadIdx.x] = inc - own;
+  }
   __syncthreads();
   Entry* list = reinterpret_cast<Entry*>(reinterpret_cast<char*>(a.ws) + kPlanHeader);
   // Offsets that overlap could name more entries than the workspace holds; the
@@ -140,7 +145,7 @@ __global__ void __launch_bounds__(kPlanThreads) fa_packed_plan_kernel(const Plan
     const int at = atomicAdd(&hist[cls], 1);
     if (at < room) list[at] = e;
   });
-  if (threadIdx.x == kPlanThreads - 1) a.ws[0] = min(before + inc, room);
+  if (threadIdx.x == kPlanClasses - 1) a.ws[0] = min(inc, room);
 }
 
 // ------------------------------------------------------------- the attention
@@ -186,34 +191,6 @@ __device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-
-// The whole warp: if a value of the masked keys [lim, hi) is not finite, the row
-// over keys [0, lim) is computed again in fp32 and written to o. Rare: only rows
-// whose result was not finite come here.
-template <typename T>
-__device__ __noinline__ void fix_row(const KernelArgs& a, const T* q, const T* k, const T* v, T* o,
-                                     int lim, int hi) {
-  const int c = (threadIdx.x & 31) * 4;
-  const bool on = c < a.D;
-  bool found = false;
-  for (int j = lim; j < hi; ++j)
-    for (int e = 0; e < 4; ++e) found = found || (on && !isfinite(to_f32<T>(v[j * a.vt + c + e])));
-  if (!__any_sync(0xffffffffu, found)) return;
-  float qf[4], acc[4] = {}, m = -INFINITY, l = 0.f;
-  for (int e = 0; e < 4; ++e) qf[e] = on ? to_f32<T>(q[c + e]) * a.scale_log2 : 0.f;
-  for (int j = 0; j < lim; ++j) {
-    float s = 0.f;
-    for (int e = 0; e < 4; ++e) s = fmaf(qf[e], on ? to_f32<T>(k[j * a.kt + c + e]) : 0.f, s);
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-    const float al = exp2f(m - base), p = exp2f(s - base);
-    m = mn;
-    l = l * al + p;
-    for (int e = 0; e < 4; ++e) acc[e] = acc[e] * al + p * (on ? to_f32<T>(v[j * a.vt + c + e]) : 0.f);
-  }
-  if (on)
-    for (int e = 0; e < 4; ++e) o[c + e] = from_f32<T>(acc[e] / l);
 }
 
 template <int D, bool BF16>
@@ -282,13 +259,10 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   // the work list is the plan kernel's
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const long long num_units = (long long)a.ws[0] * a.Hk;
+  const unsigned num_units = (unsigned)a.ws[0] * (unsigned)a.Hk;  // < 2^31: the host checks
   const Entry* list = reinterpret_cast<const Entry*>(reinterpret_cast<const char*>(a.ws) + kPlanHeader);
   // CTA c takes, in round r, unit r*grid + c (even r) or r*grid + grid-1-c (odd
   // r): with the heaviest units first this pairs heavy and light ones.
-  auto unit_at = [&](uint32_t r) -> long long {
-    return (long long)r * gridDim.x + ((r & 1) ? (gridDim.x - 1 - blockIdx.x) : blockIdx.x);
-  };
   struct Unit {
     Entry e;
     int kvh;
@@ -296,10 +270,10 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   };
   auto fetch = [&](uint32_t r) -> Unit {
     Unit u;
-    const long long at = unit_at(r);
+    const unsigned at = r * gridDim.x + ((r & 1) ? (gridDim.x - 1 - blockIdx.x) : blockIdx.x);
     u.valid = at < num_units;
     if (u.valid) {
-      const long long row = at / a.Hk;
+      const unsigned row = at / (unsigned)a.Hk;
       u.kvh = (int)(at - row * a.Hk);
       const int4* p = reinterpret_cast<const int4*>(list + row);
       // plain loads: they must not move above the wait, as invariant ones may
@@ -415,10 +389,11 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     uint32_t co[2] = {0, 0};  // outputs begun per tile
     Unit next = fetch(0);
     for (uint32_t ui = 0; next.valid && ok; ++ui) {
-      const Unit u = next;
-      next = fetch(ui + 1);
-      const int n0 = u.e.n0, n1 = u.e.n1, n = max(n0, n1);
-      if (n == 0) continue;
+      const int n0 = next.e.n0, n1 = next.e.n1, n = max(n0, n1);
+      if (n == 0) {
+        next = fetch(ui + 1);
+        continue;
+      }
       if (!mbar_wait(&bars->q_full, uq & 1, abort_flag, &g_packed_status, DEV_TIMEOUT_TMA)) break;
       ++uq;
       if (!mbar_wait(&bars->k_full[g & 1], (g >> 1) & 1, abort_flag, &g_packed_status, DEV_TIMEOUT_TMA)) break;
@@ -429,6 +404,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (n1 > 0) qk(1, g & 1);
       if (leader) mma_commit(&bars->k_empty[g & 1]);
       if (n == 1 && leader) mma_commit(&bars->q_empty);
+      next = fetch(ui + 1);  // while the tensor core works
       issued = true;
       for (int j = 0; j < n; ++j) {
         const uint32_t gj = g + j, gk = gj + 1;
@@ -513,6 +489,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     uint8_t* stg = sO + (warp - 4) * C::kOutStageBytes;
     bool ok = true;
     uint32_t gs = 0, co = 0;  // S blocks of this tile seen, outputs read
+    bool odd = false;         // a row's result may hold what its masked keys hold
     Unit next = fetch(0);
     for (uint32_t ui = 0; next.valid && ok; ++ui) {
       const Unit u = next;
@@ -637,64 +614,107 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       // no key: zeros; keys whose scores are all -inf, or NaN: NaN
       const float inv = lim <= 0 ? 0.f : l_run > 0.f ? 1.f / l_run : __int_as_float(0x7fffffff);
+      // All of the row first, so that the next unit's P.V may overwrite O early.
+      uint32_t r[D];
+      if (n_t > 0) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+          tmem_ld32(tO[t] + lane_off + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < D; ++e) asm volatile("" : "+r"(r[e]));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->o_empty[t]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < D; ++e) r[e] = 0u;
+      }
       float probe = 0.f;  // NaN once a value of the row is not finite
 #pragma unroll
       for (int at = 0; at < C::kAtoms; ++at) {
         __syncwarp();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t r[32];
-          if (n_t > 0) {
-            tmem_ld32(tO[t] + lane_off + at * 64 + c * 32, r);
-            tmem_ld_wait();
-          } else {
+        for (int v = 0; v < 8; ++v) {
+          uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) r[e] = 0u;
+          for (int e = 0; e < 4; ++e) {
+            const float f0 = __uint_as_float(r[at * 64 + v * 8 + 2 * e]) * inv;
+            const float f1 = __uint_as_float(r[at * 64 + v * 8 + 2 * e + 1]) * inv;
+            probe = fmaf(f0, 0.f, probe);
+            probe = fmaf(f1, 0.f, probe);
+            w[e] = BF16 ? pack_bf162(f0, f1) : pack_half2(f0, f1);
           }
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float f0 = __uint_as_float(r[v * 8 + 2 * e]) * inv;
-              const float f1 = __uint_as_float(r[v * 8 + 2 * e + 1]) * inv;
-              probe = fmaf(f0, 0.f, probe);
-              probe = fmaf(f1, 0.f, probe);
-              w[e] = BF16 ? pack_bf162(f0, f1) : pack_half2(f0, f1);
-            }
-            *reinterpret_cast<uint4*>(stg + lane * 128 + (((c * 4 + v) ^ (lane & 7)) * 16)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-        if (at == C::kAtoms - 1 && n_t > 0) {
-          // every TMEM read of O is done: the next P.V may overwrite it
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->o_empty[t]);
+          *reinterpret_cast<uint4*>(stg + lane * 128 + ((v ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         __syncwarp();
         // 8 lanes write a row's 128 bytes, four rows at a time
 #pragma unroll
         for (int it = 0; it < 8; ++it) {
-          const int r = it * 4 + (lane >> 3), ch = lane & 7;
-          const long long off = __shfl_sync(0xffffffffu, ooff, r);
-          const uint4 val = *reinterpret_cast<const uint4*>(stg + r * 128 + ((ch ^ (r & 7)) * 16));
+          const int line = it * 4 + (lane >> 3), ch = lane & 7;
+          const long long off = __shfl_sync(0xffffffffu, ooff, line);
+          const uint4 val = *reinterpret_cast<const uint4*>(stg + line * 128 + ((ch ^ (line & 7)) * 16));
           if (off >= 0 && at * 64 + ch * 8 < a.D)
             *reinterpret_cast<uint4*>(obase + off + at * 64 + ch * 8) = val;
         }
       }
-      if (a.causal) {
-        const int hi = min(n_t * kBN, u.e.Lk);
-        unsigned todo = __ballot_sync(0xffffffffu, live && lim > 0 && lim < hi && probe != probe);
-        while (todo) {
-          const int src = __ffs(todo) - 1;
-          todo &= todo - 1;
-          const int fi = __shfl_sync(0xffffffffu, i, src), fg = __shfl_sync(0xffffffffu, gh, src);
-          const int flim = __shfl_sync(0xffffffffu, lim, src);
-          const T* q = static_cast<const T*>(a.q) + (u.e.q0 + (long long)fi) * a.qt + ((long long)u.kvh * a.G + fg) * a.qh;
-          fix_row<T>(a, q, static_cast<const T*>(a.k) + u.e.k0 * a.kt + u.kvh * a.kh,
-                     static_cast<const T*>(a.v) + u.e.k0 * a.vt + u.kvh * a.vh,
-                     obase + __shfl_sync(0xffffffffu, ooff, src), flim, hi);
+      odd = odd || (lim > 0 && lim < min(n_t * kBN, u.e.Lk) && probe != probe);
+    }
+    if (__any_sync(0xffffffffu, odd)) {
+      // A result of this warp was not finite, in a row with masked keys in its blocks.
+      // Walk its units again: where a row is not finite and a masked value is not
+      // either, the row is computed anew in fp32. Out of the loop above, where even a
+      // call cost its registers (causal [4, 16, 2048, 128] 78 -> 85 us).
+      __syncwarp();
+      const int c = lane * 4;
+      const bool on = c < a.D;
+      auto load4 = [&](const void* base, long long at, float (&x)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = on ? to_f32<T>(static_cast<const T*>(base)[at + c + e]) : 0.f;
+      };
+      auto unfinished = [&](const float (&x)[4]) {
+        return __any_sync(0xffffffffu, !(isfinite(x[0]) && isfinite(x[1]) && isfinite(x[2]) && isfinite(x[3])));
+      };
+      for (uint32_t ui = 0;; ++ui) {
+        const Unit u = fetch(ui);
+        if (!u.valid) break;
+        const int hi = min((t == 0 ? u.e.n0 : u.e.n1) * kBN, u.e.Lk);
+        for (int x = 0; x < 32; ++x) {
+          const int w = (quarter * 32 + x) / a.G, i = t * a.R + w;
+          const int n = a.causal ? min(u.e.Lk, u.e.lim0 + i) : u.e.Lk;
+          if (w >= a.R || i >= u.e.nq || n <= 0 || n >= hi) continue;
+          const long long token = u.e.q0 + i, head = u.kvh * a.G + (quarter * 32 + x) - w * a.G;
+          const long long k0 = u.e.k0 * a.kt + u.kvh * a.kh, v0 = u.e.k0 * a.vt + u.kvh * a.vh;
+          float f[4];
+          load4(a.o, token * a.ot + head * a.oh, f);
+          if (!unfinished(f)) continue;
+          bool found = false;
+          for (int j = n; j < hi && !found; ++j) {
+            load4(a.v, v0 + j * a.vt, f);
+            found = unfinished(f);
+          }
+          if (!found) continue;
+          float q[4], acc[4] = {}, m = -INFINITY, l = 0.f;
+          load4(a.q, token * a.qt + head * a.qh, q);
+          for (int j = 0; j < n; ++j) {
+            load4(a.k, k0 + j * a.kt, f);
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = fmaf(q[e], f[e], s);
+#pragma unroll
+            for (int y = 16; y > 0; y >>= 1) s += __shfl_xor_sync(0xffffffffu, s, y);
+            s *= scale_log2;
+            const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
+            const float al = exp2f(m - base), p = exp2f(s - base);
+            m = mn;
+            l = l * al + p;
+            load4(a.v, v0 + j * a.vt, f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = acc[e] * al + p * f[e];
+          }
+          if (on)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) static_cast<T*>(a.o)[token * a.ot + head * a.oh + c + e] = from_f32<T>(acc[e] / l);
         }
       }
     }
@@ -739,7 +759,7 @@ int launch(const PackedCall& c, cudaStream_t st) {
   }
   int* ws = static_cast<int*>(c.workspace);
   const PlanArgs pa = {c.cu_q, c.cu_k, (int)c.B, (int)c.Tq, (int)c.Tk, R, c.causal, ws};
-  fa_packed_plan_kernel<<<1, kPlanThreads, 0, st>>>(pa);
+  fa_packed_plan_kernel<<<1, c.B <= 6 ? kPlanClasses : 1024, 0, st>>>(pa);  // a warp per sequence
   B2_CHECK_LAUNCH();
   KernelArgs a = {ws, c.q, c.k, c.v, c.o};
   a.qt = c.strides[0];
@@ -757,6 +777,10 @@ int launch(const PackedCall& c, cudaStream_t st) {
   a.causal = c.causal;
   a.scale_log2 = c.sm_scale * kLog2e;
   const long long most = (c.Tq / (2 * R) + c.B + 2) * c.Hk;
+  if (most >= (1LL << 31)) {
+    set_error("b2_fa_packed: %lld units of work are too many for one launch", most);
+    return B2_EINVAL;
+  }
   const int sms = device_sm_count();
   // The kernel's prologue (barriers, TMEM, descriptors) runs beside the plan kernel.
   cudaLaunchAttribute attr = {};
