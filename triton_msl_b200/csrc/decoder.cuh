@@ -2,10 +2,32 @@
 // (capi_decoder.cu) and their kernels.
 #pragma once
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
 namespace b2 {
+
+// Runs `set` (a cudaError_t call on the current device) once per device, for
+// settings such as a kernel's shared-memory limit that a launch needs every time
+// and that cost a microsecond; a failure is returned and tried again next time.
+class OncePerDevice {
+ public:
+  template <typename F>
+  cudaError_t operator()(F&& set) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done_.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = set();
+    if (e == cudaSuccess && dev < 64) done_.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
 
 // From capi.cu: the name behind b2_last_kernel(), and whether the current
 // device runs the tcgen05 kernels.

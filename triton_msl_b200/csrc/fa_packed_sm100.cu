@@ -745,18 +745,16 @@ int launch(const PackedCall& c, cudaStream_t st) {
     if (!encode_tmap(&tm[i], tdt, 3, ptrs[i], dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return B2_ELAUNCH;
   }
   auto kern = fa_packed_kernel<D, BF16>;
-  B2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<D>::kSmem));
-  {
+  static OncePerDevice ready;
+  B2_CUDA_TRY(ready([&] {
     // setmaxnreg.inc waits until the block's register pool can serve it: only
     // launch when the compiled allocation covers the split.
     cudaFuncAttributes fa;
-    B2_CUDA_TRY(cudaFuncGetAttributes(&fa, kern));
-    if (fa.numRegs < kLaunchRegs) {
-      set_error("b2_fa_packed: kernel compiled with %d registers/thread, register split needs %d",
-                fa.numRegs, kLaunchRegs);
-      return B2_ELAUNCH;
-    }
-  }
+    cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+    if (e != cudaSuccess) return e;
+    if (fa.numRegs < kLaunchRegs) return cudaErrorInvalidKernelImage;
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<D>::kSmem);
+  }));
   int* ws = static_cast<int*>(c.workspace);
   const PlanArgs pa = {c.cu_q, c.cu_k, (int)c.B, (int)c.Tq, (int)c.Tk, R, c.causal, ws};
   fa_packed_plan_kernel<<<1, c.B <= 6 ? kPlanClasses : 1024, 0, st>>>(pa);  // a warp per sequence

@@ -768,7 +768,8 @@ int launch(AttnArgs& a, cudaStream_t st) {
     return B2_EINVAL;
   }
   auto kern = kv_attn_kernel<T, D, GROUP, NT>;
-  B2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static OncePerDevice ready;
+  B2_CUDA_TRY(ready([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }));
   int grid = device_sm_count() * (NT == 1 ? 4 : 2);
   if (grid > kMaxGrid) grid = kMaxGrid;
   kern<<<grid, kThreads, smem, st>>>(a);
