@@ -8,7 +8,8 @@ import torch
 
 import triton_msl_b200 as b2
 from triton_msl_b200 import _lib
-from triton_msl_b200.decoder_ops import _I64x4, _I64x5, _I64x6, _I64x8, _I64x12
+
+_I64x4, _I64x5, _I64x6, _I64x8, _I64x12 = (ctypes.c_int64 * n for n in (4, 5, 6, 8, 12))
 
 
 # ------------------------------------------------------------------ rope_table

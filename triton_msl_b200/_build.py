@@ -4,6 +4,8 @@ Every ``csrc/*.cu`` is compiled separately with nvcc (in parallel, only when
 the source or a header changed) and linked into ``triton_msl_b200/libb2msl.so``
 with the CUDA runtime linked statically, so the library carries no dependency
 on the toolkit's shared cudart and travels with the source tree.
+``csrc/binding.cpp``, the native Python binding of the decoder-serving operators,
+is compiled against torch's headers into ``triton_msl_b200/_decoder.so``.
 """
 from __future__ import annotations
 
@@ -19,6 +21,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libb2msl.so"
+BINDING_SRC = CSRC / "binding.cpp"
+BINDING = PKG / "_decoder.so"
 INCLUDE = ROOT / "include"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -59,8 +63,35 @@ def _compile(src: Path, obj: Path, verbose: bool) -> tuple[Path, str]:
     return src, r.stdout + r.stderr
 
 
+def build_binding(force: bool = False) -> Path:
+    """Compile the native binding if its source or the C header changed. Returns its path."""
+    newest = max(p.stat().st_mtime for p in (BINDING_SRC, *INCLUDE.glob("*.h")))
+    if BINDING.exists() and not force and BINDING.stat().st_mtime >= newest:
+        return BINDING
+    import sysconfig
+
+    import torch
+    gxx = shutil.which("g++")
+    if gxx is None:
+        raise RuntimeError("g++ not found; the native binding cannot be built")
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(root / "include"), "-I", str(root / "include/torch/csrc/api/include"),
+           "-I", sysconfig.get_paths()["include"], "-I", str(cuda / "include"), str(BINDING_SRC), "-o", str(tmp),
+           "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compile and link libb2msl.so if anything changed. Returns the library path."""
+    """Compile and link libb2msl.so and the native binding if anything changed. Returns
+    the library's path."""
     BUILD.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
     hdr_mtime = max((h.stat().st_mtime for h in _headers()), default=0.0)
@@ -87,6 +118,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
     if verbose:
         for name, log in sorted(logs.items()):
             print(f"== {name}\n{log}", file=sys.stderr)
+    build_binding(force)
     return LIB
 
 

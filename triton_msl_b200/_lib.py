@@ -16,6 +16,7 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("B2MSL_LIBRARY", PKG / "libb2msl.so"))
+BINDING_PATH = PKG / "_decoder.so"  # native binding of decoder_ops
 
 B2_OK, B2_EINVAL, B2_EUNSUPPORTED, B2_ELAUNCH, B2_ETIMEOUT = 0, -1, -2, -3, -4
 B2_F32, B2_F16, B2_BF16, B2_I64, B2_I32 = 0, 1, 2, 3, 4
@@ -93,6 +94,16 @@ class B2Unsupported(B2Error, NotImplementedError):
     """The request is valid but not implemented (B2_EUNSUPPORTED)."""
 
 
+def autobuild() -> bool:
+    """Whether a missing library is built on first use."""
+    return os.environ.get("B2MSL_NO_AUTOBUILD") != "1"
+
+
+def address(fn) -> int:
+    """The address of an entry point of lib()."""
+    return ctypes.cast(fn, ctypes.c_void_p).value
+
+
 def lib() -> ctypes.CDLL:
     """Load (building in-tree first if absent and nvcc exists) and return the library."""
     global _lib
@@ -100,7 +111,7 @@ def lib() -> ctypes.CDLL:
         return _lib
     with _lock:
         if _lib is None:
-            if not LIB_PATH.exists() and os.environ.get("B2MSL_NO_AUTOBUILD") != "1":
+            if not LIB_PATH.exists() and autobuild():
                 from . import _build
                 _build.build()
             if not LIB_PATH.exists():
