@@ -289,7 +289,8 @@ int b2_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, cons
  *     word i*(D/64)+g of the row;
  *   k_scales, v_scales: bf16 [pages, H, page_size, D/group, 2] = (scale, low).
  * A code c stands for c*scale + low, with low = min of the group rounded down to
- * bf16, scale = (max - low)/15 rounded up to bf16 and c = rint((x - low)/scale).
+ * bf16, scale = (max - low) * (1/15) rounded up to bf16 and, each operation in
+ * fp32, c = rint((x - low) * (1/scale)).
  * A group that holds a NaN or an infinity reads back as NaN.
  * Slot s is token s % page_size of page s / page_size.
  *

@@ -216,6 +216,25 @@ def test_cache_write_and_read(dtype, T, H, D, group, page):
             assert torch.equal(got, row_values(codes, scales).float().to(out))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_cache_codes_follow_their_definition(dtype):
+    # bit for bit in fp32, values half way between two codes among them (in 16 bits there are many)
+    g = gen(8)
+    cache = b2.kv_cache_alloc(64, 4, 128, 16, 64)
+    x = (torch.round(randn(g, 1000, 4, 128) * 16) / 8).to(dtype)
+    slots = torch.arange(1000, device="cuda")
+    b2.kv_cache_write(cache, x, -x, slots)
+    kc, ks, vc, vs = pick(cache, slots)
+    halves = 0
+    for y, codes, scales in ((x, kc, ks), (-x, vc, vs)):
+        y = y.float().unflatten(-1, (2, 64))
+        step, low = scales[..., :1].float(), scales[..., 1:].float()
+        quotient = (y - low) * (1.0 / step)
+        halves += (quotient % 1 == 0.5).sum().item()
+        assert torch.equal(row_codes(codes).unflatten(-1, (2, 64)), torch.round(quotient).long())
+    assert halves > 100
+
+
 def test_cache_strides_and_alignment():
     g = gen(5)
     T, H, D = 19, 3, 64

@@ -145,8 +145,11 @@ __device__ __forceinline__ uint32_t quantise(const T (&x)[8], uint32_t& meta) {
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     f2_t y = f2_add(f2_pack(to_f32<T>(x[i]), to_f32<T>(x[i + 1])), f2_pack(-low, -low));
-    y = f2_add(f2_mul(y, f2_pack(inv, inv)), f2_pack(12582912.0f, 12582912.0f));
     float y0, y1;
+    f2_unpack(y, y0, y1);
+    // the product is rounded by itself: a packed product and sum come out fused, which
+    // decides values half way between two codes differently
+    y = f2_add(f2_pack(__fmul_rn(y0, inv), __fmul_rn(y1, inv)), f2_pack(12582912.0f, 12582912.0f));
     f2_unpack(y, y0, y1);
     word += (__float_as_uint(y0) << (4 * i)) + (__float_as_uint(y1) << (4 * i + 4));
     bias += (kMagic << (4 * i)) + (kMagic << (4 * i + 4));
