@@ -34,6 +34,20 @@ class OncePerDevice {
 void set_last_kernel(const char* name);
 bool device_is_sm100();
 
+// Division by a number known at launch, n < 2^31: a multiply and a shift in place of
+// the twenty instructions of a 32-bit division (Granlund and Montgomery 1994).
+struct FastDiv {
+  uint32_t d = 1, mul = 1, shift = 0;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t by) : d(by) {
+    while ((1ull << shift) < by) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+#endif
+};
+
 struct RopeCall {
   const void *q, *k;
   void *qo, *ko;

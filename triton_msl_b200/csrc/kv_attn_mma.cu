@@ -19,7 +19,7 @@
 //
 // Work is split along the keys: all sequences' tiles of 128 keys form one line that
 // is cut evenly among the CTAs (four per SM), whatever the lengths. Inside a tile
-// each of 4 warps takes 32 keys in two steps. A warp's codes and scales come by
+// each of 4 warps takes 32 keys. A warp's codes and scales come by
 // cp.async into its own two buffers of shared memory, so no barrier is needed in the
 // loop. At a sequence's end, or the CTA's, the warps' partial results are merged; a
 // sequence cut between CTAs is joined by kv_attn_join_kernel from partials in the
@@ -101,8 +101,11 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
 }
 __device__ __forceinline__ int tiles_of(const AttnArgs& a, int b) { return (keys_of(a, b) + kTile - 1) / kTile; }
 
-// The line of all tiles: sequence after sequence, in each segment after segment (key
-// head, block of rows). CTA c of n holds tiles [share * c + min(c, more), ...).
+// The line of all work: sequence after sequence, in each segment after segment (key
+// head, block of rows), a segment kSetup units for its start and end, then its tiles.
+// CTA c of n holds units [share * c + min(c, more), ...). Measured on 32 sequences of
+// up to 2048 / 8192 keys: kSetup 0: 22.1 / 48.5 us, 1: 19.0 / 45.1, 2: 18.6 / 44.1.
+constexpr int kSetup = 2;
 struct Line {
   unsigned share, more, ctas;
   __device__ Line(unsigned total, unsigned grid) {
@@ -111,17 +114,18 @@ struct Line {
     more = total - share * ctas;
   }
   __device__ unsigned begin(unsigned c) const { return share * c + min(c, more); }
-  __device__ unsigned owner(unsigned tile) const {
+  __device__ unsigned owner(unsigned unit) const {
     const unsigned big = more * (share + 1);
-    return tile < big ? tile / (share + 1) : more + (tile - big) / share;
+    return unit < big ? unit / (share + 1) : more + (unit - big) / share;
   }
 };
-// Tiles per segment of all sequences, and of those before b; the whole warp.
-__device__ __forceinline__ unsigned count_tiles(const AttnArgs& a, int b, unsigned* before) {
+__device__ __forceinline__ unsigned units_of(int tiles) { return tiles ? tiles + kSetup : 0; }
+// Units per segment of all sequences, and of those before b; the whole warp.
+__device__ __forceinline__ unsigned count_units(const AttnArgs& a, int b, unsigned* before) {
   unsigned all = 0, some = 0;
 #pragma unroll 4
   for (int i = threadIdx.x & 31; i < a.B; i += 32) {
-    const unsigned n = tiles_of(a, i);
+    const unsigned n = units_of(tiles_of(a, i));
     all += n;
     if (i < b) some += n;
   }
@@ -152,19 +156,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
 
   // ---- this CTA's part of the line of all tiles; every warp finds it by itself
   asm volatile("griddepcontrol.launch_dependents;");
-  const Line line(count_tiles(a, 0, nullptr) * segs, gridDim.x);
+  const Line line(count_units(a, 0, nullptr) * segs, gridDim.x);
   if (blockIdx.x >= line.ctas) return;
   const unsigned begin = line.begin(blockIdx.x), end = line.begin(blockIdx.x + 1);
   // The segment at hand: sequence, key head and block of rows.
   struct Segment {
     int b, kvh, rb, keys, tiles;
   } sg = {};
-  int tile = 0;  // its first tile here
+  int at = 0;  // the unit of it at which this CTA begins
   {
     unsigned base = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       const int keys = b0 + lane < a.B ? keys_of(a, b0 + lane) : 0;
-      const unsigned n = (unsigned)((keys + kTile - 1) / kTile) * segs;
+      const unsigned n = units_of((keys + kTile - 1) / kTile) * segs;
       unsigned inc = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -178,16 +182,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
         sg.keys = __shfl_sync(0xffffffffu, keys, w);
         const unsigned first = base + __shfl_sync(0xffffffffu, inc - n, w);
         sg.tiles = (sg.keys + kTile - 1) / kTile;
-        const int seg = (int)((begin - first) / sg.tiles);
+        const int seg = (int)((begin - first) / units_of(sg.tiles));
         sg.kvh = a.row_blocks == 1 ? seg : seg / a.row_blocks;
         sg.rb = seg - sg.kvh * a.row_blocks;
-        tile = (int)(begin - first) - seg * sg.tiles;
+        at = (int)(begin - first) - seg * (int)units_of(sg.tiles);
         break;
       }
       base += __shfl_sync(0xffffffffu, inc, 31);
     }
   }
-  int left = (int)(end - begin);  // tiles of this CTA
+  int left = (int)(end - begin);  // units of this CTA
 
   // ---- loads, one tile ahead
   uint8_t* ring = smem + warp * (kStages * kSteps * R::kStage);
@@ -340,92 +344,95 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
   const int k_off = g * (D / 2) + t * (D / 8), m_off = R::kKScales + g * NG * 4;
   const int v_off = R::kVCodes + v_place<D>(2 * t, D == 128 ? g >> 1 : g >> 2) + (D == 128 ? (g & 1) * 8 : (g & 3) * 4);
 
-  // ---- 16 keys
+  // ---- 32 keys: two times 16, whose instructions fill one another's waits
   auto step = [&](const uint8_t* st, int key0, int keys) {
-    // scores
-    uint32_t k0[WPT], k1[WPT], km[2][NG], vm[2][NG];
-    if constexpr (D == 128) {
-      *reinterpret_cast<uint4*>(k0) = *reinterpret_cast<const uint4*>(st + k_off);
-      *reinterpret_cast<uint4*>(k1) = *reinterpret_cast<const uint4*>(st + k_off + 8 * (D / 2));
-    } else {
-      *reinterpret_cast<uint2*>(k0) = *reinterpret_cast<const uint2*>(st + k_off);
-      *reinterpret_cast<uint2*>(k1) = *reinterpret_cast<const uint2*>(st + k_off + 8 * (D / 2));
-    }
+    float x[kSteps][NT][4], sv[kSteps][2][NG], lv[kSteps][2][NG];  // x: scores less the running maximum
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint8_t* p = st + m_off + 8 * h * NG * 4;
-      if constexpr (NG == 2) {
-        *reinterpret_cast<uint2*>(km[h]) = *reinterpret_cast<const uint2*>(p);
-        *reinterpret_cast<uint2*>(vm[h]) = *reinterpret_cast<const uint2*>(p + R::kScales);
+    for (int u = 0; u < kSteps; ++u) {
+      const uint8_t* p0 = st + u * R::kStage;
+      uint32_t k0[WPT], k1[WPT], km[2][NG], vm[2][NG];
+      if constexpr (D == 128) {
+        *reinterpret_cast<uint4*>(k0) = *reinterpret_cast<const uint4*>(p0 + k_off);
+        *reinterpret_cast<uint4*>(k1) = *reinterpret_cast<const uint4*>(p0 + k_off + 8 * (D / 2));
       } else {
-        km[h][0] = *reinterpret_cast<const uint32_t*>(p);
-        vm[h][0] = *reinterpret_cast<const uint32_t*>(p + R::kScales);
+        *reinterpret_cast<uint2*>(k0) = *reinterpret_cast<const uint2*>(p0 + k_off);
+        *reinterpret_cast<uint2*>(k1) = *reinterpret_cast<const uint2*>(p0 + k_off + 8 * (D / 2));
       }
-    }
-    float acc[NG][NT][4] = {};
-#pragma unroll
-    for (int w = 0; w < WPT; ++w)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const uint32_t x0 = s ? k0[w] >> 8 : k0[w], x1 = s ? k1[w] >> 8 : k1[w];
-        const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu;
-        const uint32_t a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          mma16816(acc[NG == 2 ? w % N64 : 0][nt], a0, a1, a2, a3, qf[nt][w][s][0], qf[nt][w][s][1]);
-      }
-    float x[NT][4], sv[2][NG], lv[2][NG];  // scores less the running maximum
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        sv[h][k] = scale_of(vm[h][k]);
-        lv[h][k] = low_of(vm[h][k]);
-      }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int h = i >> 1, c2 = i & 1;
-        float u = scale_of(km[h][0]) * acc[0][nt][i], y = fmaf(low_of(km[h][0]), qs[nt][0][c2], -m[nt][c2]);
-        if constexpr (NG == 2) {
-          u = fmaf(scale_of(km[h][1]), acc[1][nt][i], u);
-          y = fmaf(low_of(km[h][1]), qs[nt][1][c2], y);
-        }
-        x[nt][i] = fmaf(u, f[nt][c2], y);
-      }
-    const bool edge = key0 + 16 > keys_all;  // some row keeps only a part
-    if (edge) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int key = key0 + g + 8 * h;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c2 = 0; c2 < 2; ++c2)
-            if (key >= lim[nt][c2]) x[nt][2 * h + c2] = -INFINITY;
-        // past the sequence the page holds anything
-        if (key >= keys)
-#pragma unroll
-          for (int k = 0; k < NG; ++k) sv[h][k] = lv[h][k] = 0.f;
+        const uint8_t* p = p0 + m_off + 8 * h * NG * 4;
+        if constexpr (NG == 2) {
+          *reinterpret_cast<uint2*>(km[h]) = *reinterpret_cast<const uint2*>(p);
+          *reinterpret_cast<uint2*>(vm[h]) = *reinterpret_cast<const uint2*>(p + R::kScales);
+        } else {
+          km[h][0] = *reinterpret_cast<const uint32_t*>(p);
+          vm[h][0] = *reinterpret_cast<const uint32_t*>(p + R::kScales);
+        }
       }
+      float acc[NG][NT][4] = {};
+#pragma unroll
+      for (int w = 0; w < WPT; ++w)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t x0 = s ? k0[w] >> 8 : k0[w], x1 = s ? k1[w] >> 8 : k1[w];
+          const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu;
+          const uint32_t a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816(acc[NG == 2 ? w % N64 : 0][nt], a0, a1, a2, a3, qf[nt][w][s][0], qf[nt][w][s][1]);
+        }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          sv[u][h][k] = scale_of(vm[h][k]);
+          lv[u][h][k] = low_of(vm[h][k]);
+        }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int h = i >> 1, c2 = i & 1;
+          float w = scale_of(km[h][0]) * acc[0][nt][i], y = fmaf(low_of(km[h][0]), qs[nt][0][c2], -m[nt][c2]);
+          if constexpr (NG == 2) {
+            w = fmaf(scale_of(km[h][1]), acc[1][nt][i], w);
+            y = fmaf(low_of(km[h][1]), qs[nt][1][c2], y);
+          }
+          x[u][nt][i] = fmaf(w, f[nt][c2], y);
+        }
+    }
+    const bool edge = key0 + 16 * kSteps > keys_all;  // some row keeps only a part
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < kSteps; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = key0 + 16 * u + g + 8 * h;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c2 = 0; c2 < 2; ++c2)
+              if (key >= lim[nt][c2]) x[u][nt][2 * h + c2] = -INFINITY;
+          // past the sequence the page, or a buffer that nothing was loaded into,
+          // holds anything
+          if (key >= keys)
+#pragma unroll
+            for (int k = 0; k < NG; ++k) sv[u][h][k] = lv[u][h][k] = 0.f;
+        }
     }
     // raise the maxima, or lower F, where needed
-    float svf[2][NG];
+    float top_sv = 0.f;  // NaN is left aside
 #pragma unroll
-    for (int k = 0; k < NG; ++k) {
-      svf[0][k] = sv[0][k] * F;
-      svf[1][k] = sv[1][k] * F;
-    }
-    float over = fmaxf(svf[0][0], svf[1][0]);
-    if constexpr (NG == 2) over = max3(over, svf[0][1], svf[1][1]);
+    for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) over = max3(over, max3(x[nt][0], x[nt][1], x[nt][2]), x[nt][3]);
+      for (int k = 0; k < NG; ++k) top_sv = max3(top_sv, sv[u][0][k], sv[u][1][k]);
+    float over = top_sv * F;
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) over = max3(over, max3(x[u][nt][0], x[u][nt][1], x[u][nt][2]), x[u][nt][3]);
     if (__any_sync(0xffffffffu, over > 8.f) || fresh) {
-      float top = 0.f;
-#pragma unroll
-      for (int k = 0; k < NG; ++k) top = fmaxf(top, fmaxf(sv[0][k], sv[1][k]));  // NaN is left aside
-      const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+      const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top_sv));
       float ratio = 1.f;
       if (__uint_as_float(top_bits) * F > 8.f) {  // to 4 .. 8
         const float to = __int_as_float(min(max(256 - (int)(top_bits >> 23), 1), 254) << 23);
@@ -436,15 +443,20 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c2 = 0; c2 < 2; ++c2) {
-          float y = fmaxf(x[nt][c2], x[nt][2 + c2]);
+          float y = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < kSteps; ++u) y = max3(y, x[u][nt][c2], x[u][nt][2 + c2]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
           // the maximum's step; the first keys may set it below its start of 0
           const float up = fresh ? (y > -INFINITY ? y : 0.f) : fmaxf(y, 0.f);
           const float al = ex2(-up);
           m[nt][c2] += up;
-          x[nt][c2] -= up;
-          x[nt][2 + c2] -= up;
+#pragma unroll
+          for (int u = 0; u < kSteps; ++u) {
+            x[u][nt][c2] -= up;
+            x[u][nt][2 + c2] -= up;
+          }
           l[nt][c2] *= al;
 #pragma unroll
           for (int k = 0; k < NG; ++k) lo[nt][k][c2] *= al;
@@ -454,85 +466,86 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
             o[i][nt][2 + c2] *= al * ratio;
           }
         }
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        svf[0][k] = sv[0][k] * F;
-        svf[1][k] = sv[1][k] * F;
-      }
       fresh = false;
     }
-    // weights, and their products with the values' scales as the B operand
     // F is a power of two: 1/F by its exponent
     const float mid = 7.5f * __int_as_float((254 << 23) - __float_as_int(F));
-    uint32_t pf[NT][NG][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float p[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = ex2(x[nt][i]);
-        l[nt][i & 1] += p[i];
-      }
+    for (int u = 0; u < kSteps; ++u) {
+      // weights, and their products with the values' scales as the B operand
+      uint32_t pf[NT][NG][2];
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
-        float w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = p[i] * svf[i >> 1][k];
-        if (edge) {
-          // a row's own masked keys count for nothing, NaN or not
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool out = key0 + g + 8 * (i >> 1) >= lim[nt][i & 1];
-            if (out) w[i] = 0.f;
-            lo[nt][k][i & 1] += out ? 0.f : p[i] * lv[i >> 1][k];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) lo[nt][k][i & 1] = fmaf(p[i], lv[i >> 1][k], lo[nt][k][i & 1]);
-        }
-        uint32_t packed[2] = {half2_bits(w[0], w[1]), half2_bits(w[2], w[3])};
-        if constexpr (std::is_same<T, __half>::value) {
-          // What the rounding took from a weight, times the middle of the codes, goes
-          // to the lowest values' sum: the rounding then counts for the code's distance
-          // from 7.5 and not for the whole code. fp16 results resolve that (error of 16
-          // sequences of up to 4095 keys 4.5e-4 -> MEASURE); bf16 ones do not.
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&packed[h]));
-            lo[nt][k][0] = fmaf(w[2 * h] - r.x, mid, lo[nt][k][0]);
-            lo[nt][k][1] = fmaf(w[2 * h + 1] - r.y, mid, lo[nt][k][1]);
-          }
-        }
-        pf[nt][k][0] = transpose8(packed[0]);
-        pf[nt][k][1] = transpose8(packed[1]);
+        sv[u][0][k] *= F;
+        sv[u][1][k] *= F;
       }
-    }
-    // values
-    uint32_t vw[4][N64];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {  // keys 2t + (i & 1) + 8 (i >> 1): v_place keeps their distances
-      const uint8_t* p = st + v_off + ((i & 1) * 4 + (i >> 1) * 8) * (D / 2);
-      if constexpr (D == 128) *reinterpret_cast<uint2*>(vw[i]) = *reinterpret_cast<const uint2*>(p);
-      else vw[i][0] = *reinterpret_cast<const uint32_t*>(p);
-    }
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
 #pragma unroll
-    for (int w = 0; w < N64; ++w) {
-      uint32_t y[4];  // keys 2t, 2t+1, 2t+8, 2t+9: channels 64w + 8g ..
+        for (int i = 0; i < 4; ++i) {
+          p[i] = ex2(x[u][nt][i]);
+          l[nt][i & 1] += p[i];
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = vw[i][w];
+        for (int k = 0; k < NG; ++k) {
+          float w[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {  // codes 4h .. 4h+3 of each word
-        uint32_t p0 = __byte_perm(y[0], y[1], h ? 0x7632 : 0x5410);
-        uint32_t p1 = __byte_perm(y[2], y[3], h ? 0x7632 : 0x5410);
+          for (int i = 0; i < 4; ++i) w[i] = p[i] * sv[u][i >> 1][k];
+          if (edge) {
+            // a row's own masked keys count for nothing, NaN or not
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const uint32_t a0 = p0 & 0x000f000fu, a1 = p0 & 0x00f000f0u;
-          const uint32_t a2 = p1 & 0x000f000fu, a3 = p1 & 0x00f000f0u;
+            for (int i = 0; i < 4; ++i) {
+              const bool out = key0 + 16 * u + g + 8 * (i >> 1) >= lim[nt][i & 1];
+              if (out) w[i] = 0.f;
+              lo[nt][k][i & 1] += out ? 0.f : p[i] * lv[u][i >> 1][k];
+            }
+          } else {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816(o[w * 4 + 2 * h + s][nt], a0, a1, a2, a3, pf[nt][NG == 2 ? w : 0][0], pf[nt][NG == 2 ? w : 0][1]);
-          p0 >>= 8;
-          p1 >>= 8;
+            for (int i = 0; i < 4; ++i) lo[nt][k][i & 1] = fmaf(p[i], lv[u][i >> 1][k], lo[nt][k][i & 1]);
+          }
+          uint32_t packed[2] = {half2_bits(w[0], w[1]), half2_bits(w[2], w[3])};
+          if constexpr (std::is_same<T, __half>::value) {
+            // What the rounding took from a weight, times the middle of the codes, goes
+            // to the lowest values' sum: the rounding then counts for the code's distance
+            // from 7.5 and not for the whole code. fp16 results resolve that (16 sequences
+            // of up to 4095 keys: relative error 4.5e-4 without, 2.8e-4 with, 2.1e-4 of it
+            // the output's rounding); bf16 ones do not.
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&packed[h]));
+              lo[nt][k][0] = fmaf(w[2 * h] - r.x, mid, lo[nt][k][0]);
+              lo[nt][k][1] = fmaf(w[2 * h + 1] - r.y, mid, lo[nt][k][1]);
+            }
+          }
+          pf[nt][k][0] = transpose8(packed[0]);
+          pf[nt][k][1] = transpose8(packed[1]);
+        }
+      }
+      // values
+      uint32_t vw[4][N64];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // keys 2t + (i & 1) + 8 (i >> 1): v_place keeps their distances
+        const uint8_t* p = st + u * R::kStage + v_off + ((i & 1) * 4 + (i >> 1) * 8) * (D / 2);
+        if constexpr (D == 128) *reinterpret_cast<uint2*>(vw[i]) = *reinterpret_cast<const uint2*>(p);
+        else vw[i][0] = *reinterpret_cast<const uint32_t*>(p);
+      }
+#pragma unroll
+      for (int w = 0; w < N64; ++w) {  // channels 64w + 8g ..
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // codes 4h .. 4h+3 of each word
+          uint32_t p0 = __byte_perm(vw[0][w], vw[1][w], h ? 0x7632 : 0x5410);
+          uint32_t p1 = __byte_perm(vw[2][w], vw[3][w], h ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const uint32_t a0 = p0 & 0x000f000fu, a1 = p0 & 0x00f000f0u;
+            const uint32_t a2 = p1 & 0x000f000fu, a3 = p1 & 0x00f000f0u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(o[w * 4 + 2 * h + s][nt], a0, a1, a2, a3, pf[nt][NG == 2 ? w : 0][0], pf[nt][NG == 2 ? w : 0][1]);
+            p0 >>= 8;
+            p1 >>= 8;
+          }
         }
       }
     }
@@ -612,43 +625,41 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
 
   // ---- the segments of this CTA's part of the line
   while (true) {
-    const int start = tile;
-    const int stop = min(sg.tiles, tile + left);
-    {
-      const size_t head = (size_t)sg.kvh * a.page_size;
-      k_src = a.k_codes + head * (D / 2) + lane * 16;
-      v_src = a.v_codes + head * (D / 2) + lane * 16;
-      s_src = reinterpret_cast<const uint8_t*>(lane < kPieces ? a.k_scales : a.v_scales) + head * (NG * 4) + (lane % kPieces) * 16;
-      pages = a.page_table + sg.b * a.table_stride;
-    }
-    wrong = false;
-    left -= stop - tile;
-    lookup(tile);
-    load_rows(sg);
-    load(tile, 0);
-    if (tile + 1 < stop) lookup(tile + 1);
-    begin_segment(sg);
-    int stage = 0;
-    for (; tile < stop; ++tile) {
-      cp_async_wait<0>();
-      __syncwarp();  // the other lanes' pieces have landed, and all are done with the other buffer
-      if (tile + 1 < stop) {
-        load(tile + 1, stage ^ 1);
-        if (tile + 2 < stop) lookup(tile + 2);
+    const int until = min((int)units_of(sg.tiles), at + left);
+    left -= until - at;
+    const int start = max(0, at - kSetup), stop = max(0, until - kSetup);  // tiles
+    if (start < stop) {
+      {
+        const size_t head = (size_t)sg.kvh * a.page_size;
+        k_src = a.k_codes + head * (D / 2) + lane * 16;
+        v_src = a.v_codes + head * (D / 2) + lane * 16;
+        s_src = reinterpret_cast<const uint8_t*>(lane < kPieces ? a.k_scales : a.v_scales) + head * (NG * 4) + (lane % kPieces) * 16;
+        pages = a.page_table + sg.b * a.table_stride;
       }
-#pragma unroll 1
-      for (int s = 0; s < kSteps; ++s) {
-        const int key0 = tile * kTile + (warp * kSteps + s) * 16;
-        if (key0 >= sg.keys) break;
-        step(ring + (stage * kSteps + s) * R::kStage, key0, sg.keys);
+      wrong = false;
+      lookup(start);
+      load_rows(sg);
+      load(start, 0);
+      if (start + 1 < stop) lookup(start + 1);
+      begin_segment(sg);
+      int stage = 0;
+      for (int tile = start; tile < stop; ++tile) {
+        cp_async_wait<0>();
+        __syncwarp();  // the other lanes' pieces have landed, and all are done with the other buffer
+        if (tile + 1 < stop) {
+          load(tile + 1, stage ^ 1);
+          if (tile + 2 < stop) lookup(tile + 2);
+        }
+        const int key0 = tile * kTile + warp * kSteps * 16;
+        if (key0 < sg.keys) step(ring + stage * kSteps * R::kStage, key0, sg.keys);
+        stage ^= 1;
       }
-      stage ^= 1;
+      if (wrong && lane == 0) atomicOr(a.status, DEV_BAD_INDEX);
+      end_segment(sg, start > 0, stop < sg.tiles);
     }
-    if (wrong && lane == 0) atomicOr(a.status, DEV_BAD_INDEX);
-    end_segment(sg, start > 0, stop < sg.tiles);
     if (left == 0) break;
     // the next segment that has tiles
-    tile = 0;
+    at = 0;
     if (++sg.rb == a.row_blocks) {
       sg.rb = 0;
       if (++sg.kvh == a.H) {
@@ -691,8 +702,8 @@ __global__ void __launch_bounds__(kJoin) kv_attn_join_kernel(const __grid_consta
     return;
   }
   unsigned before;
-  const Line line(count_tiles(a, b, &before) * segs, grid);
-  before = before * segs + (unsigned)seg * tiles;
+  const Line line(count_units(a, b, &before) * segs, grid);
+  before = before * segs + (unsigned)seg * units_of(tiles) + kSetup;  // the first tile
   const int c0 = (int)line.owner(before), c1 = (int)line.owner(before + tiles - 1);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (c0 == c1) return;  // whole in one CTA, which wrote it
@@ -762,7 +773,7 @@ int launch(AttnArgs& a, cudaStream_t st) {
   constexpr int ROWS = 8 * NT;
   constexpr size_t smem = (size_t)kWarps * kStages * kSteps * R::kStage + (size_t)kWarps * ROWS * (D + 6) * sizeof(float);
   a.row_blocks = (a.rows + ROWS - 1) / ROWS;
-  const double tiles = (double)a.B * a.H * a.row_blocks * (((double)a.max_pages * a.page_size + kTile) / kTile);
+  const double tiles = (double)a.B * a.H * a.row_blocks * (((double)a.max_pages * a.page_size + kTile) / kTile + kSetup);
   if (tiles >= 2147483648.0) {
     set_error("b2_kv_cache_attn: B * H * row blocks * (max_pages * page_size / %d) must be < 2^31", kTile);
     return B2_EINVAL;

@@ -16,8 +16,10 @@
 // of every 64-channel group and each tensor-core step stays inside one group
 // (kv_attn.cu). Scales [pages, H, page, D/group, 2].
 //
-// Bound: HBM. One thread owns one word of keys and the same word of values; a
-// group's extremes take 3 or 4 shuffles.
+// Bound: HBM and, for 16-bit rows, instructions. One thread owns two words of keys and
+// the same two of values: a group's extremes, scale and reciprocal are then found by 4
+// or 8 lanes (8 or 16 with one word a thread: a write of 32768 tokens of 8 heads of 128 took
+// 42 us where it takes 29, 5.9 TB/s; the read back 35, 4.9 TB/s).
 #include <type_traits>
 
 #include "b2_common.cuh"
@@ -56,49 +58,47 @@ struct RowsArgs {
   const void* slots;
   long long kt, kh, vt, vh;
   unsigned rows, H, page_size, capacity;
+  FastDiv by_heads, by_page;
   int slots64;
 };
 
-// 8 values of one row, as they come
+// A lane's channels of one row: two words of 8.
+constexpr int kPer = 16;
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, T (&x)[8]) {
+__device__ __forceinline__ void load_row(const T* p, T (&x)[kPer]) {
   if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(p)[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p[i];
+    for (int i = 0; i < kPer; ++i) x[i] = p[i];
   }
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, const T (&x)[8]) {
-  if constexpr (VEC) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(x)[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = x[i];
-  }
-}
-
 __device__ __forceinline__ __nv_bfloat162 max2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2_nan(a, b); }
 __device__ __forceinline__ __half2 max2(__half2 a, __half2 b) { return __hmax2_nan(a, b); }
+__device__ __forceinline__ __nv_bfloat162 min2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmin2_nan(a, b); }
+__device__ __forceinline__ __half2 min2(__half2 a, __half2 b) { return __hmin2_nan(a, b); }
 
 __device__ __forceinline__ __nv_bfloat162 low_pair(__nv_bfloat162 a, __nv_bfloat162 b) { return __lows2bfloat162(a, b); }
 __device__ __forceinline__ __half2 low_pair(__half2 a, __half2 b) { return __lows2half2(a, b); }
 __device__ __forceinline__ __nv_bfloat162 high_pair(__nv_bfloat162 a, __nv_bfloat162 b) { return __highs2bfloat162(a, b); }
 __device__ __forceinline__ __half2 high_pair(__half2 a, __half2 b) { return __highs2half2(a, b); }
 
-// Largest and lowest value of a group of LANES * 8 values; NaN when it holds one.
+// Largest and lowest value of a group of LANES * 16 values; NaN when it holds one.
 // 16-bit types: compared two at a time in their own type, (max, -min) in one word, so
 // that one shuffle and one packed maximum serve both (every step is exact).
 template <int LANES, typename T>
-__device__ __forceinline__ void extremes(const T (&x)[8], float& hi, float& lo) {
+__device__ __forceinline__ void extremes(const T (&x)[kPer], float& hi, float& lo) {
   if constexpr (sizeof(T) == 2) {
     using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
     const T2* p = reinterpret_cast<const T2*>(x);
-    T2 up = max2(max2(p[0], p[1]), max2(p[2], p[3]));
-    T2 dn = max2(max2(__hneg2(p[0]), __hneg2(p[1])), max2(__hneg2(p[2]), __hneg2(p[3])));
+    T2 up = p[0], dn = p[0];
+#pragma unroll
+    for (int i = 1; i < kPer / 2; ++i) {
+      up = max2(up, p[i]);
+      dn = min2(dn, p[i]);
+    }
+    dn = __hneg2(dn);
     T2 m = max2(low_pair(up, dn), high_pair(up, dn));
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) {
@@ -110,7 +110,7 @@ __device__ __forceinline__ void extremes(const T (&x)[8], float& hi, float& lo) 
   } else {
     hi = lo = x[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
+    for (int i = 1; i < kPer; ++i) {
       hi = max_nan(hi, x[i]);
       lo = fminf(lo, x[i]);
     }
@@ -122,9 +122,9 @@ __device__ __forceinline__ void extremes(const T (&x)[8], float& hi, float& lo) 
   }
 }
 
-// The code word of 8 values and the group's (scale, lo) as two packed bf16.
+// The code words of 16 values and the group's (scale, lo) as two packed bf16.
 template <int LANES, typename T>
-__device__ __forceinline__ uint32_t quantise(const T (&x)[8], uint32_t& meta) {
+__device__ __forceinline__ void quantise(const T (&x)[kPer], uint32_t (&word)[2], uint32_t& meta) {
   float hi, lo;
   extremes<LANES>(x, hi, lo);
   const float low = bf16_down(lo);
@@ -132,70 +132,82 @@ __device__ __forceinline__ uint32_t quantise(const T (&x)[8], uint32_t& meta) {
   const float scale = bf16_up(step);
   if (!(step < INFINITY) || !(scale < INFINITY)) {  // a NaN or an infinity in the group
     meta = 0x7fff7fffu;
-    return 0u;
+    word[0] = word[1] = 0u;
+    return;
   }
   meta = (__float_as_uint(scale) >> 16) | (__float_as_uint(low) & 0xffff0000u);
   // below 2^-126 the reciprocal may overflow; the group reads back as lo then
-  const float inv = scale >= 1.17549435e-38f ? 1.0f / scale : 0.0f;
+  const float inv = scale >= 1.17549435e-38f ? __frcp_rn(scale) : 0.0f;
   // (x - low) * inv is at most 15 (1 + 2^-21), scale being rounded up. Adding
   // 1.5 * 2^23 rounds it to the nearest integer (ties to even) and leaves that in
   // the low bits; what the constant's own bits add to the word is subtracted.
   constexpr uint32_t kMagic = 0x4b400000u;
-  uint32_t word = 0, bias = 0;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    f2_t y = f2_add(f2_pack(to_f32<T>(x[i]), to_f32<T>(x[i + 1])), f2_pack(-low, -low));
-    float y0, y1;
-    f2_unpack(y, y0, y1);
-    // the product is rounded by itself: a packed product and sum come out fused, which
-    // decides values half way between two codes differently
-    y = f2_add(f2_pack(__fmul_rn(y0, inv), __fmul_rn(y1, inv)), f2_pack(12582912.0f, 12582912.0f));
-    f2_unpack(y, y0, y1);
-    word += (__float_as_uint(y0) << (4 * i)) + (__float_as_uint(y1) << (4 * i + 4));
-    bias += (kMagic << (4 * i)) + (kMagic << (4 * i + 4));
+  for (int w = 0; w < 2; ++w) {
+    uint32_t sum = 0, bias = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      f2_t y = f2_add(f2_pack(to_f32<T>(x[8 * w + i]), to_f32<T>(x[8 * w + i + 1])), f2_pack(-low, -low));
+      float y0, y1;
+      f2_unpack(y, y0, y1);
+      // the product is rounded by itself: a packed product and sum come out fused,
+      // which decides values half way between two codes differently
+      y = f2_add(f2_pack(__fmul_rn(y0, inv), __fmul_rn(y1, inv)), f2_pack(12582912.0f, 12582912.0f));
+      f2_unpack(y, y0, y1);
+      sum += (__float_as_uint(y0) << (4 * i)) + (__float_as_uint(y1) << (4 * i + 4));
+      bias += (kMagic << (4 * i)) + (kMagic << (4 * i + 4));
+    }
+    word[w] = sum - bias;
   }
-  return word - bias;
 }
 
+// Where the lane's first word lies in the row; its second is D/64 further.
 template <int D>
 __device__ __forceinline__ int stored_word(int lane) {
-  return (lane & 7) * (D / 64) + (lane >> 3);
+  return (lane & 3) * 2 * (D / 64) + (lane >> 2);
 }
 
 template <typename T, int D, int GROUP, bool VEC>
 __global__ void __launch_bounds__(kCacheThreads) kv_write_kernel(const __grid_constant__ RowsArgs a) {
-  constexpr int LPR = D / 8;
+  constexpr int LPR = D / kPer, LPG = GROUP / kPer;  // lanes of a row, of a group
   const unsigned tid = blockIdx.x * kCacheThreads + threadIdx.x;
   const unsigned row = tid / LPR;
   const int lane = tid % LPR;
   // threads past the last row repeat it without storing: the shuffles need them
   const unsigned r = row < a.rows ? row : a.rows - 1;
-  const unsigned token = r / a.H, head = r - token * a.H;
-  __align__(16) T k[8], v[8];
-  load8<T, VEC>(static_cast<const T*>(a.k) + (long long)token * a.kt + (long long)head * a.kh + lane * 8, k);
-  load8<T, VEC>(static_cast<const T*>(a.v) + (long long)token * a.vt + (long long)head * a.vh + lane * 8, v);
+  const unsigned token = a.by_heads.div(r), head = r - token * a.H;
+  __align__(16) T k[kPer], v[kPer];
+  load_row<T, VEC>(static_cast<const T*>(a.k) + (long long)token * a.kt + (long long)head * a.kh + lane * kPer, k);
+  load_row<T, VEC>(static_cast<const T*>(a.v) + (long long)token * a.vt + (long long)head * a.vh + lane * kPer, v);
   const long long slot = a.slots64 ? static_cast<const long long*>(a.slots)[token]
                                    : static_cast<const int*>(a.slots)[token];
-  uint32_t mk, mv;
-  const uint32_t wk = quantise<GROUP / 8>(k, mk), wv = quantise<GROUP / 8>(v, mv);
+  uint32_t mk, mv, wk[2], wv[2];
+  quantise<LPG>(k, wk, mk);
+  quantise<LPG>(v, wv, mv);
   if (row >= a.rows || slot < 0) return;
   if (slot >= (long long)a.capacity) {
     if (lane == 0) atomicOr(&g_kv_cache_status, DEV_BAD_INDEX);
     return;
   }
-  const unsigned page = (unsigned)slot / a.page_size, place = (unsigned)slot - page * a.page_size;
+  const unsigned page = a.by_page.div((unsigned)slot), place = (unsigned)slot - page * a.page_size;
   const size_t at = ((size_t)page * a.H + head) * a.page_size + place;
-  a.k_codes[at * LPR + stored_word<D>(lane)] = wk;
-  a.v_codes[at * LPR + stored_word<D>(lane)] = wv;
-  if (lane % (GROUP / 8) == 0) {
-    a.k_scales[at * (D / GROUP) + lane / (GROUP / 8)] = mk;
-    a.v_scales[at * (D / GROUP) + lane / (GROUP / 8)] = mv;
+  uint32_t* kc = a.k_codes + at * (D / 8) + stored_word<D>(lane);
+  uint32_t* vc = a.v_codes + at * (D / 8) + stored_word<D>(lane);
+  kc[0] = wk[0];
+  kc[D / 64] = wk[1];
+  vc[0] = wv[0];
+  vc[D / 64] = wv[1];
+  if (lane % LPG == 0) {
+    a.k_scales[at * (D / GROUP) + lane / LPG] = mk;
+    a.v_scales[at * (D / GROUP) + lane / LPG] = mv;
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void values8(uint32_t word, uint32_t meta, T (&x)[8]) {
+// The 8 values of one word.
+template <typename T, bool VEC>
+__device__ __forceinline__ void put_values(T* p, uint32_t word, uint32_t meta) {
   const float s = __uint_as_float(meta << 16), lo = __uint_as_float(meta & 0xffff0000u);
+  __align__(16) T x[8];
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     // 2^23 + c minus 2^23 is the code as a float
@@ -207,42 +219,61 @@ __device__ __forceinline__ void values8(uint32_t word, uint32_t meta, T (&x)[8])
     x[i] = from_f32<T>(y0);
     x[i + 1] = from_f32<T>(y1);
   }
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(x)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = x[i];
+  }
 }
 
+// A lane takes two words that are stored side by side, of one group (D = 64) or of two.
 template <typename T, int D, int GROUP, bool VEC>
 __global__ void __launch_bounds__(kCacheThreads) kv_read_kernel(const __grid_constant__ RowsArgs a) {
-  constexpr int LPR = D / 8;
+  constexpr int LPR = D / kPer, NG = D / GROUP;
   const unsigned tid = blockIdx.x * kCacheThreads + threadIdx.x;
   const unsigned row = tid / LPR;
   const int lane = tid % LPR;
   if (row >= a.rows) return;
-  const unsigned token = row / a.H, head = row - token * a.H;
+  const unsigned token = a.by_heads.div(row), head = row - token * a.H;
   const long long slot = a.slots64 ? static_cast<const long long*>(a.slots)[token]
                                    : static_cast<const int*>(a.slots)[token];
-  __align__(16) T k[8], v[8];
+  T* k = static_cast<T*>(a.k) + (long long)token * a.kt + (long long)head * a.kh;
+  T* v = static_cast<T*>(a.v) + (long long)token * a.vt + (long long)head * a.vh;
+  const int c0 = D == 128 ? 8 * lane : 16 * lane, c1 = D == 128 ? 64 + 8 * lane : 16 * lane + 8;
   if (slot >= 0 && slot < (long long)a.capacity) {
-    const unsigned page = (unsigned)slot / a.page_size, place = (unsigned)slot - page * a.page_size;
+    const unsigned page = a.by_page.div((unsigned)slot), place = (unsigned)slot - page * a.page_size;
     const size_t at = ((size_t)page * a.H + head) * a.page_size + place;
-    const uint32_t wk = a.k_codes[at * LPR + stored_word<D>(lane)];
-    const uint32_t wv = a.v_codes[at * LPR + stored_word<D>(lane)];
-    const uint32_t mk = a.k_scales[at * (D / GROUP) + lane / (GROUP / 8)];
-    const uint32_t mv = a.v_scales[at * (D / GROUP) + lane / (GROUP / 8)];
-    values8(wk, mk, k);
-    values8(wv, mv, v);
+    const uint2 wk = reinterpret_cast<const uint2*>(a.k_codes)[at * LPR + lane];
+    const uint2 wv = reinterpret_cast<const uint2*>(a.v_codes)[at * LPR + lane];
+    uint2 mk, mv;
+    if constexpr (NG == 2) {
+      mk = reinterpret_cast<const uint2*>(a.k_scales)[at];
+      mv = reinterpret_cast<const uint2*>(a.v_scales)[at];
+    } else {
+      mk.x = mk.y = a.k_scales[at];
+      mv.x = mv.y = a.v_scales[at];
+    }
+    put_values<T, VEC>(k + c0, wk.x, mk.x);
+    put_values<T, VEC>(k + c1, wk.y, mk.y);
+    put_values<T, VEC>(v + c0, wv.x, mv.x);
+    put_values<T, VEC>(v + c1, wv.y, mv.y);
   } else {
-    // a negative slot is padding and reads as zero; one past the cache as NaN
-    const float fill = slot < 0 ? 0.f : __int_as_float(0x7fffffff);
+    // a negative slot is padding and reads as zero; one past the cache as NaN: scale 0,
+    // lowest value 0 or NaN
+    const uint32_t fill = slot < 0 ? 0u : 0x7fff0000u;
     if (slot >= 0 && lane == 0) atomicOr(&g_kv_cache_status, DEV_BAD_INDEX);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) k[i] = v[i] = from_f32<T>(fill);
+    put_values<T, VEC>(k + c0, 0u, fill);
+    put_values<T, VEC>(k + c1, 0u, fill);
+    put_values<T, VEC>(v + c0, 0u, fill);
+    put_values<T, VEC>(v + c1, 0u, fill);
   }
-  store8<T, VEC>(static_cast<T*>(a.k) + (long long)token * a.kt + (long long)head * a.kh + lane * 8, k);
-  store8<T, VEC>(static_cast<T*>(a.v) + (long long)token * a.vt + (long long)head * a.vh + lane * 8, v);
 }
 
 template <bool WRITE, typename T, int D, int GROUP>
 int launch(const RowsArgs& a, bool vec, cudaStream_t st) {
-  const unsigned long long threads = (unsigned long long)a.rows * (D / 8);
+  const unsigned long long threads = (unsigned long long)a.rows * (D / kPer);
   const unsigned grid = (unsigned)((threads + kCacheThreads - 1) / kCacheThreads);
   if constexpr (WRITE) {
     if (vec) kv_write_kernel<T, D, GROUP, true><<<grid, kCacheThreads, 0, st>>>(a);
@@ -282,6 +313,8 @@ int rows_launch(const CacheRowsCall& c, cudaStream_t st) {
   a.H = (unsigned)s.H;
   a.page_size = (unsigned)s.page_size;
   a.capacity = (unsigned)(s.pages * s.page_size);
+  a.by_heads = FastDiv(a.H);
+  a.by_page = FastDiv(a.page_size);
   const long long per = 16 / dtype_size(c.dtype);
   const bool vec = ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15) == 0 &&
                    a.kt % per == 0 && a.kh % per == 0 && a.vt % per == 0 && a.vh % per == 0;

@@ -57,6 +57,7 @@ struct RopeArgs {
   const void* positions;
   long long P;
   unsigned items;        // lane groups per token (both tensors)
+  FastDiv by_items;
   unsigned items_q;      // of these, the queries'
   unsigned total;        // items * tokens
   int pos64, D, R, log_tpr, heads_per_group;
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kRopeThreads, 3) rope_kernel(const __grid_cons
   const int lane = threadIdx.x & (tpr - 1);
   // Lanes past the last group stay for the shuffles and load nothing.
   const bool live = gid < a.total;
-  const unsigned token = live ? gid / a.items : 0;
+  const unsigned token = live ? a.by_items.div(gid) : 0;
   const unsigned item = live ? gid - token * a.items : 0;
   const bool is_k = item >= a.items_q;
   const RopeTensor& in = a.in[is_k ? 1 : 0];
@@ -305,11 +306,12 @@ int launch(RopeArgs& a, long long tokens, bool inter, cudaStream_t st) {
   a.items = a.items_q + (unsigned)((a.in[1].heads + per - 1) / per);
   const long long total = tokens * a.items;
   const long long threads = total << a.log_tpr;
-  if (threads + kRopeThreads >= (1LL << 32)) {
+  if (threads + kRopeThreads >= (1LL << 32) || total >= (1LL << 31)) {
     set_error("b2_qk_norm_rope: %lld tokens x %u lane groups are too many for one launch", tokens, a.items);
     return B2_EINVAL;
   }
   a.total = (unsigned)total;
+  a.by_items = FastDiv(a.items);
   const unsigned grid = (unsigned)((threads + kRopeThreads - 1) / kRopeThreads);
   if (inter) rope_kernel<T, VE, NP, true><<<grid, kRopeThreads, 0, st>>>(a);
   else rope_kernel<T, VE, NP, false><<<grid, kRopeThreads, 0, st>>>(a);
