@@ -25,6 +25,7 @@
 #include "b2_common.cuh"
 #include "decoder.cuh"
 #include "fa_math.cuh"
+#include "vec16.cuh"
 
 namespace b2 {
 namespace {
@@ -147,8 +148,14 @@ __device__ __forceinline__ void quantise(const T (&x)[kPer], uint32_t (&word)[2]
     uint32_t sum = 0, bias = 0;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      f2_t y = f2_add(f2_pack(to_f32<T>(x[8 * w + i]), to_f32<T>(x[8 * w + i + 1])), f2_pack(-low, -low));
       float y0, y1;
+      if constexpr (sizeof(T) == 2) {
+        widen2<T>(reinterpret_cast<const uint32_t*>(x)[4 * w + i / 2], y0, y1);
+      } else {
+        y0 = x[8 * w + i];
+        y1 = x[8 * w + i + 1];
+      }
+      f2_t y = f2_add(f2_pack(y0, y1), f2_pack(-low, -low));
       f2_unpack(y, y0, y1);
       // the product is rounded by itself: a packed product and sum come out fused,
       // which decides values half way between two codes differently
@@ -216,8 +223,12 @@ __device__ __forceinline__ void put_values(T* p, uint32_t word, uint32_t meta) {
     y = f2_fma(f2_add(y, f2_pack(-8388608.0f, -8388608.0f)), f2_pack(s, s), f2_pack(lo, lo));
     float y0, y1;
     f2_unpack(y, y0, y1);
-    x[i] = from_f32<T>(y0);
-    x[i + 1] = from_f32<T>(y1);
+    if constexpr (sizeof(T) == 2) {
+      reinterpret_cast<uint32_t*>(x)[i / 2] = narrow2<T>(y0, y1);
+    } else {
+      x[i] = y0;
+      x[i + 1] = y1;
+    }
   }
   if constexpr (VEC) {
 #pragma unroll

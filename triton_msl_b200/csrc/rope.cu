@@ -12,16 +12,16 @@
 // and the norm one shuffle tree; the lane's table values are loaded once for
 // all four heads, whose loads are issued together before any arithmetic.
 // 16-bit inputs are bound by instructions as much as by HBM (converting, norm and
-// rotation take about ten a value): vectors of 4 channels, 16 lanes a head of 128,
-// leave registers for 24 warps per SM; with vectors of 8, 16 warps, it took 92 us
-// where it takes 81 now (16384 tokens, 32 + 8 heads of 128, bf16: 4.2 TB/s; fp32
-// 104 us, 6.5 TB/s).
-// The arithmetic is fp32 throughout; only the result is rounded to x's type.
+// rotation, 16 a value): vectors of 4 channels, 16 lanes a head of 128, leave
+// registers for 24 warps per SM. Measured on 16384 tokens, 32 + 8 heads of 128, norm,
+// half layout: bf16 74 us, 4.7 TB/s (vectors of 8, 16 warps, and a division per head
+// in the norm: 92); fp32 102 us, 6.6 TB/s.
 #include <type_traits>
 
 #include "b2_common.cuh"
 #include "decoder.cuh"
 #include "fa_math.cuh"
+#include "vec16.cuh"
 
 namespace b2 {
 namespace {
@@ -38,9 +38,9 @@ template <> struct RawVec<8> { using type = uint2; };
 template <> struct RawVec<4> { using type = uint32_t; };
 template <> struct RawVec<2> { using type = uint16_t; };
 
-// Heads per lane group, and CTAs per SM below: measured on 16384 tokens of 32 + 8
-// heads of 128, bf16 with norm, 4 heads and 3 CTAs (80 registers) 81 us; 2 heads and
-// 4 CTAs 91; 2 and 5 83; 4 and 4 (64 registers, spills) 110.
+// Heads per lane group, and CTAs per SM below. When they were chosen (the same case),
+// 4 heads and 3 CTAs (80 registers) took 81 us; 2 heads and 4 CTAs 91; 2 and 5 83; 4
+// and 4 (64 registers, spills) 110.
 constexpr int kHeads = 4;
 
 struct RopeTensor {
@@ -56,10 +56,10 @@ struct RopeArgs {
   const float* table;    // [P, R]: cos | sin
   const void* positions;
   long long P;
-  unsigned items;        // lane groups per token (both tensors)
-  FastDiv by_items;
-  unsigned items_q;      // of these, the queries'
-  unsigned total;        // items * tokens
+  unsigned blocks_q;     // CTAs of the queries; the keys' follow
+  unsigned groups[2];    // lane groups of each tensor
+  unsigned items[2];     // of a token
+  FastDiv by_items[2];
   int pos64, D, R, log_tpr, heads_per_group;
   float eps, inv_dim;
 };
@@ -110,22 +110,68 @@ __device__ __forceinline__ Vals<VE> fma(const Vals<VE>& a, const Vals<VE>& b, co
   return r;
 }
 
+// The first and second values of a unit's pairs from its two vectors, and back.
+template <typename T, int VE, bool INTER, typename Raw>
+__device__ __forceinline__ void widen(const Raw (&x)[2], float (&a)[VE], float (&b)[VE]) {
+  if constexpr (sizeof(T) == 2 && VE % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      if constexpr (INTER) widen2<T>(w[e], a[e], b[e]);
+      else if (e % 2 == 0) {
+        widen2<T>(w[e / 2], a[e], a[e + 1]);
+        widen2<T>(w[(VE + e) / 2], b[e], b[e + 1]);
+      }
+    }
+  } else {
+    const T* v = reinterpret_cast<const T*>(x);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      a[e] = to_f32<T>(v[INTER ? 2 * e : e]);
+      b[e] = to_f32<T>(v[INTER ? 2 * e + 1 : VE + e]);
+    }
+  }
+}
+template <typename T, int VE, bool INTER, typename Raw>
+__device__ __forceinline__ void narrow(const float (&a)[VE], const float (&b)[VE], Raw (&x)[2]) {
+  if constexpr (sizeof(T) == 2 && VE % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(x);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      if constexpr (INTER) w[e] = narrow2<T>(a[e], b[e]);
+      else if (e % 2 == 0) {
+        w[e / 2] = narrow2<T>(a[e], a[e + 1]);
+        w[(VE + e) / 2] = narrow2<T>(b[e], b[e + 1]);
+      }
+    }
+  } else {
+    T* v = reinterpret_cast<T*>(x);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      v[INTER ? 2 * e : e] = from_f32<T>(a[e]);
+      v[INTER ? 2 * e + 1 : VE + e] = from_f32<T>(b[e]);
+    }
+  }
+}
+
 // One lane holds NP units of 2*VE values of each head. Unit u < R/(2 VE) is
 // rotated: channels [u VE, u VE + VE) with those R/2 above (half layout), or the
 // 2 VE neighbours from 2 u VE (interleaved). The other units are copied.
-template <typename T, int VE, int NP, bool INTER>
+// TPR lanes share a head (0: 1 << log_tpr).
+template <typename T, int VE, int NP, int TPR, bool INTER>
 __global__ void __launch_bounds__(kRopeThreads, 3) rope_kernel(const __grid_constant__ RopeArgs a) {
   using Raw = typename RawVec<VE * (int)sizeof(T)>::type;
-  const int tpr = 1 << a.log_tpr;
-  const unsigned gid = (blockIdx.x * kRopeThreads + threadIdx.x) >> a.log_tpr;
+  const int tpr = TPR ? TPR : 1 << a.log_tpr;
+  // A CTA has heads of one tensor, so what belongs to the tensor is uniform in it.
+  const int which = blockIdx.x >= a.blocks_q ? 1 : 0;
+  const RopeTensor& in = a.in[which];
+  const unsigned tid = (blockIdx.x - (which ? a.blocks_q : 0)) * kRopeThreads + threadIdx.x;
+  const unsigned gid = TPR ? tid / TPR : tid >> a.log_tpr;
   const int lane = threadIdx.x & (tpr - 1);
   // Lanes past the last group stay for the shuffles and load nothing.
-  const bool live = gid < a.total;
-  const unsigned token = live ? a.by_items.div(gid) : 0;
-  const unsigned item = live ? gid - token * a.items : 0;
-  const bool is_k = item >= a.items_q;
-  const RopeTensor& in = a.in[is_k ? 1 : 0];
-  const int h0 = (int)(is_k ? item - a.items_q : item) * a.heads_per_group;
+  const bool live = gid < a.groups[which];
+  const unsigned token = live ? a.by_items[which].div(gid) : 0;
+  const int h0 = live ? (int)(gid - token * a.items[which]) * a.heads_per_group : 0;
   const int nh = live ? min(a.heads_per_group, in.heads - h0) : 0;
   const T* x = static_cast<const T*>(in.x) + (long long)token * in.xt + (long long)h0 * in.xh;
   T* y = static_cast<T*>(in.y) + (long long)token * in.yt + (long long)h0 * in.yh;
@@ -221,19 +267,12 @@ __global__ void __launch_bounds__(kRopeThreads, 3) rope_kernel(const __grid_cons
 #pragma unroll
   for (int i = 0; i < kHeads; ++i)
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const T* x0 = reinterpret_cast<const T*>(raw[i][p]);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        va[i][p][e] = to_f32<T>(x0[INTER ? 2 * e : e]);
-        vb[i][p][e] = to_f32<T>(x0[INTER ? 2 * e + 1 : VE + e]);
-      }
-    }
+    for (int p = 0; p < NP; ++p) widen<T, VE, INTER>(raw[i][p], va[i][p], vb[i][p]);
   // 1/rms of each head; the heads' shuffle trees run beside one another
   float r[kHeads];
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) r[i] = 1.f;
-  if (a.in[0].w || a.in[1].w) {  // the whole grid alike, so every lane takes part
+  if (w) {  // the whole CTA alike, so every lane takes part
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
       Vals<VE> s2;
@@ -256,7 +295,7 @@ __global__ void __launch_bounds__(kRopeThreads, 3) rope_kernel(const __grid_cons
 #pragma unroll
         for (int i = 0; i < kHeads; ++i) r[i] += __shfl_xor_sync(0xffffffffu, r[i], o);
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) r[i] = w ? rsqrtf(fmaf(r[i], a.inv_dim, a.eps)) : 1.f;
+    for (int i = 0; i < kHeads; ++i) r[i] = rsqrtf(fmaf(r[i], a.inv_dim, a.eps));
   }
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
@@ -279,12 +318,7 @@ __global__ void __launch_bounds__(kRopeThreads, 3) rope_kernel(const __grid_cons
       mul(ya, scale).get(oa);
       mul(yb, scale).get(ob);
       Raw out[2];
-      T* e0 = reinterpret_cast<T*>(out);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        e0[INTER ? 2 * e : e] = from_f32<T>(oa[e]);
-        e0[INTER ? 2 * e + 1 : VE + e] = from_f32<T>(ob[e]);
-      }
+      narrow<T, VE, INTER>(oa, ob, out);
       *reinterpret_cast<Raw*>(y0 + i * yh) = out[0];
       *reinterpret_cast<Raw*>(y0 + i * yh + gap) = out[1];
     }
@@ -302,19 +336,29 @@ int launch(RopeArgs& a, long long tokens, bool inter, cudaStream_t st) {
   a.log_tpr = 0;
   while ((1 << a.log_tpr) < units && a.log_tpr < 5) ++a.log_tpr;
   a.heads_per_group = per;
-  a.items_q = (unsigned)((a.in[0].heads + per - 1) / per);
-  a.items = a.items_q + (unsigned)((a.in[1].heads + per - 1) / per);
-  const long long total = tokens * a.items;
-  const long long threads = total << a.log_tpr;
-  if (threads + kRopeThreads >= (1LL << 32) || total >= (1LL << 31)) {
-    set_error("b2_qk_norm_rope: %lld tokens x %u lane groups are too many for one launch", tokens, a.items);
-    return B2_EINVAL;
+  unsigned blocks[2];
+  for (int i = 0; i < 2; ++i) {
+    a.items[i] = (unsigned)((a.in[i].heads + per - 1) / per);
+    const long long groups = tokens * a.items[i], threads = groups << a.log_tpr;
+    if (groups >= (1LL << 31) || threads + kRopeThreads >= (1LL << 32)) {
+      set_error("b2_qk_norm_rope: %lld tokens x %u lane groups are too many for one launch", tokens, a.items[i]);
+      return B2_EINVAL;
+    }
+    a.groups[i] = (unsigned)groups;
+    a.by_items[i] = FastDiv(a.items[i] ? a.items[i] : 1);
+    blocks[i] = (unsigned)((threads + kRopeThreads - 1) / kRopeThreads);
   }
-  a.total = (unsigned)total;
-  a.by_items = FastDiv(a.items);
-  const unsigned grid = (unsigned)((threads + kRopeThreads - 1) / kRopeThreads);
-  if (inter) rope_kernel<T, VE, NP, true><<<grid, kRopeThreads, 0, st>>>(a);
-  else rope_kernel<T, VE, NP, false><<<grid, kRopeThreads, 0, st>>>(a);
+  a.blocks_q = blocks[0];
+  const unsigned grid = blocks[0] + blocks[1];
+  auto run = [&](auto kernel) { kernel<<<grid, kRopeThreads, 0, st>>>(a); };
+  // The widths of a head of 64 and of 128 in vectors of four are known to the compiler.
+  if constexpr (VE == 4 && NP == 1) {
+    if (a.log_tpr == 4) run(inter ? rope_kernel<T, 4, 1, 16, true> : rope_kernel<T, 4, 1, 16, false>);
+    else if (a.log_tpr == 3) run(inter ? rope_kernel<T, 4, 1, 8, true> : rope_kernel<T, 4, 1, 8, false>);
+    else run(inter ? rope_kernel<T, 4, 1, 0, true> : rope_kernel<T, 4, 1, 0, false>);
+  } else {
+    run(inter ? rope_kernel<T, VE, NP, 0, true> : rope_kernel<T, VE, NP, 0, false>);
+  }
   B2_CHECK_LAUNCH();
   return B2_OK;
 }
