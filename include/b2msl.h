@@ -114,7 +114,8 @@ const char* b2_last_error(void);
 /* Kernel family the calling thread's last successful call launched
  * ("fa_sm100", "fa_simt", "gemm_sm100" (128x256 tiles), "gemm_sm100_n128"
  * (128x128 tiles), "gemm_sm100_pair" (256x256 tiles on CTA pairs), "gemm_sm100_splitk", "gemm_sm100_tf32x3", "gemm_simt",
- * "row_reduce", "row_split", "row_memset"). Introspection for tests and benchmarks; the reference's
+ * "row_reduce", "row_split", "row_memset", "qk_norm_rope", "kv_cache_write",
+ * "kv_cache_read", "kv_attn_mma", "kv_attn_row", "fa_packed_sm100", "fa_packed_simt"). Introspection for tests and benchmarks; the reference's
  * equivalent is its TRITON_MSL_PATH_LOG lowering-path log
  * (triton_msl/codegen/msl_emitter.py:523-538). */
 const char* b2_last_kernel(void);

@@ -159,7 +159,7 @@ __device__ __forceinline__ void narrow(const float (&a)[VE], const float (&b)[VE
 // 2 VE neighbours from 2 u VE (interleaved). The other units are copied.
 // TPR lanes share a head (0: 1 << log_tpr).
 template <typename T, int VE, int NP, int TPR, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads, 3) rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, NP == 1 ? 3 : 1) rope_kernel(const __grid_constant__ RopeArgs a) {
   using Raw = typename RawVec<VE * (int)sizeof(T)>::type;
   const int tpr = TPR ? TPR : 1 << a.log_tpr;
   // A CTA has heads of one tensor, so what belongs to the tensor is uniform in it.
