@@ -142,10 +142,14 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 // One row of the group: its token among the new ones and its query head.
 __device__ __forceinline__ int row_token(const AttnArgs& a, int row) { return row / a.G; }
 
-template <typename T, int D, int GROUP, int NT>
+// NT tiles of 8 columns (query rows). COLS = 2: every column is a row, a lane has two of
+// each tile. COLS = 1, for at most 4 rows: rows are the even columns, so that a lane has
+// one live column and the scores, exponentials and weights of the dead one are not
+// computed (half of that work for the common 4 heads on a key head).
+template <typename T, int D, int GROUP, int NT, int COLS>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(const __grid_constant__ AttnArgs a) {
   using R = Ring<D, GROUP>;
-  constexpr int NG = R::NG, N64 = D / 64, WPT = D / 32, ROWS = 8 * NT;
+  constexpr int NG = R::NG, N64 = D / 64, WPT = D / 32, ROWS = COLS * 4 * NT;
   extern __shared__ __align__(16) uint8_t smem[];
   float* s_o = reinterpret_cast<float*>(smem + kWarps * kStages * kSteps * R::kStage);  // [warp][row][D + 4]
   float* s_m = s_o + kWarps * ROWS * (D + 4);                                  // [warp][row]
@@ -238,9 +242,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
 
   // ---- a segment's state
   uint32_t qf[NT][WPT][2][2];          // B operands: code word, low or high byte pair, register
-  float f[NT][2], qs[NT][NG][2];       // per column: factor of the code part, scaled sums of q
-  int lim[NT][2];                      // keys each column's row keeps
-  float m[NT][2], l[NT][2], lo[NT][NG][2];  // running maximum, sums
+  float f[NT][COLS], qs[NT][NG][COLS]; // per column: factor of the code part, scaled sums of q
+  int lim[NT][COLS];                   // keys each column's row keeps
+  float m[NT][COLS], l[NT][COLS], lo[NT][NG][COLS];  // running maximum, sums
   float o[N64 * 4][NT][4];
   float F = 0.f;
   int keys_all = 0;                    // keys that every row keeps
@@ -250,8 +254,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
   auto load_rows = [&](const Segment& c) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = c.rb * ROWS + nt * 8 + g;
-      const bool live = row < a.rows;
+      const int row = COLS == 2 ? c.rb * ROWS + nt * 8 + g : g >> 1;
+      const bool live = row < a.rows && (COLS == 2 || g % 2 == 0);
       const int n = live ? row_token(a, row) : 0;
       const T* q = static_cast<const T*>(a.q) + (long long)c.b * a.qb + n * a.qn +
                    (long long)(c.kvh * a.G + (live ? row : 0) - n * a.G) * a.qh + 16 * t;
@@ -318,12 +322,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
           }
       // to the lanes that hold the row's scores: columns 2t, 2t + 1
 #pragma unroll
-      for (int c2 = 0; c2 < 2; ++c2) {
+      for (int c2 = 0; c2 < COLS; ++c2) {
         const int src = (2 * t + c2) * 4;
         f[nt][c2] = __shfl_sync(0xffffffffu, down, src) * (16777216.f * a.scale_log2);
 #pragma unroll
         for (int k = 0; k < NG; ++k) qs[nt][k][c2] = __shfl_sync(0xffffffffu, sum[k], src) * a.scale_log2;
-        const int r = rb * ROWS + nt * 8 + 2 * t + c2;
+        const int r = COLS == 2 ? rb * ROWS + nt * 8 + 2 * t + c2 : t;
         // rows that do not exist keep what the last token keeps
         lim[nt][c2] = r < a.rows ? max(0, c.keys - a.N + 1 + row_token(a, r)) : c.keys;
         m[nt][c2] = 0.f;
@@ -391,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; i += 3 - COLS) {
           const int h = i >> 1, c2 = i & 1;
           float w = scale_of(km[h][0]) * acc[0][nt][i], y = fmaf(low_of(km[h][0]), qs[nt][0][c2], -m[nt][c2]);
           if constexpr (NG == 2) {
@@ -411,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c2 = 0; c2 < 2; ++c2)
+            for (int c2 = 0; c2 < COLS; ++c2)
               if (key >= lim[nt][c2]) x[u][nt][2 * h + c2] = -INFINITY;
           // past the sequence the page, or a buffer that nothing was loaded into,
           // holds anything
@@ -430,7 +434,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
 #pragma unroll
     for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) over = max3(over, max3(x[u][nt][0], x[u][nt][1], x[u][nt][2]), x[u][nt][3]);
+      for (int nt = 0; nt < NT; ++nt) {
+        over = max3(over, x[u][nt][0], x[u][nt][2]);
+        if constexpr (COLS == 2) over = max3(over, x[u][nt][1], x[u][nt][3]);
+      }
     if (__any_sync(0xffffffffu, over > 8.f) || fresh) {
       const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top_sv));
       float ratio = 1.f;
@@ -442,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c2 = 0; c2 < 2; ++c2) {
+        for (int c2 = 0; c2 < COLS; ++c2) {
           float y = -INFINITY;
 #pragma unroll
           for (int u = 0; u < kSteps; ++u) y = max3(y, x[u][nt][c2], x[u][nt][2 + c2]);
@@ -483,26 +490,26 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
       for (int nt = 0; nt < NT; ++nt) {
         float p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; i += 3 - COLS) {
           p[i] = ex2(x[u][nt][i]);
           l[nt][i & 1] += p[i];
         }
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
-          float w[4];
+          float w[4] = {};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = p[i] * sv[u][i >> 1][k];
+          for (int i = 0; i < 4; i += 3 - COLS) w[i] = p[i] * sv[u][i >> 1][k];
           if (edge) {
             // a row's own masked keys count for nothing, NaN or not
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 4; i += 3 - COLS) {
               const bool out = key0 + 16 * u + g + 8 * (i >> 1) >= lim[nt][i & 1];
               if (out) w[i] = 0.f;
               lo[nt][k][i & 1] += out ? 0.f : p[i] * lv[u][i >> 1][k];
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lo[nt][k][i & 1] = fmaf(p[i], lv[u][i >> 1][k], lo[nt][k][i & 1]);
+            for (int i = 0; i < 4; i += 3 - COLS) lo[nt][k][i & 1] = fmaf(p[i], lv[u][i >> 1][k], lo[nt][k][i & 1]);
           }
           uint32_t packed[2] = {half2_bits(w[0], w[1]), half2_bits(w[2], w[3])};
           if constexpr (std::is_same<T, __half>::value) {
@@ -515,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
             for (int h = 0; h < 2; ++h) {
               const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&packed[h]));
               lo[nt][k][0] = fmaf(w[2 * h] - r.x, mid, lo[nt][k][0]);
-              lo[nt][k][1] = fmaf(w[2 * h + 1] - r.y, mid, lo[nt][k][1]);
+              if constexpr (COLS == 2) lo[nt][k][1] = fmaf(w[2 * h + 1] - r.y, mid, lo[nt][k][1]);
             }
           }
           pf[nt][k][0] = transpose8(packed[0]);
@@ -557,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int c2 = 0; c2 < 2; ++c2) {
+      for (int c2 = 0; c2 < COLS; ++c2) {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
           l[nt][c2] += __shfl_xor_sync(0xffffffffu, l[nt][c2], d);
@@ -565,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(cons
           for (int k = 0; k < NG; ++k) lo[nt][k][c2] += __shfl_xor_sync(0xffffffffu, lo[nt][k][c2], d);
         }
         if (wrong) l[nt][c2] = __int_as_float(0x7fffffff);  // no such page: the rows are undefined
-        const int r = nt * 8 + 2 * t + c2;
+        const int r = COLS == 2 ? nt * 8 + 2 * t + c2 : t;
         if (g == 0) {
           s_m[warp * ROWS + r] = l[nt][c2] == 0.f ? kNoMax : m[nt][c2];
           s_l[warp * ROWS + r] = l[nt][c2];
@@ -767,10 +774,10 @@ __global__ void __launch_bounds__(kJoin) kv_attn_join_kernel(const __grid_consta
 constexpr int kMaxGrid = 4 * 160;  // CTAs that the workspace has room for
 static_assert(kMaxGrid <= kJoinMax, "a segment's parts");
 
-template <typename T, int D, int GROUP, int NT>
+template <typename T, int D, int GROUP, int NT, int COLS>
 int launch(AttnArgs& a, cudaStream_t st) {
   using R = Ring<D, GROUP>;
-  constexpr int ROWS = 8 * NT;
+  constexpr int ROWS = COLS * 4 * NT;
   constexpr size_t smem = (size_t)kWarps * kStages * kSteps * R::kStage + (size_t)kWarps * ROWS * (D + 6) * sizeof(float);
   a.row_blocks = (a.rows + ROWS - 1) / ROWS;
   const double tiles = (double)a.B * a.H * a.row_blocks * (((double)a.max_pages * a.page_size + kTile) / kTile + kSetup);
@@ -778,7 +785,7 @@ int launch(AttnArgs& a, cudaStream_t st) {
     set_error("b2_kv_cache_attn: B * H * row blocks * (max_pages * page_size / %d) must be < 2^31", kTile);
     return B2_EINVAL;
   }
-  auto kern = kv_attn_kernel<T, D, GROUP, NT>;
+  auto kern = kv_attn_kernel<T, D, GROUP, NT, COLS>;
   static OncePerDevice ready;
   B2_CUDA_TRY(ready([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }));
   int grid = device_sm_count() * (NT == 1 ? 4 : 2);
@@ -798,15 +805,20 @@ int launch(AttnArgs& a, cudaStream_t st) {
   return B2_OK;
 }
 
+template <typename T, int D, int GROUP>
+int launch_rows(AttnArgs& a, cudaStream_t st) {
+  if (a.rows <= 4) return launch<T, D, GROUP, 1, 1>(a, st);
+  if (a.rows <= 8) return launch<T, D, GROUP, 1, 2>(a, st);
+  if constexpr (D == 64) {  // the registers of D = 128 hold two tiles at most
+    if (a.rows > 16) return launch<T, D, GROUP, 4, 2>(a, st);
+  }
+  return launch<T, D, GROUP, 2, 2>(a, st);
+}
+
 template <typename T>
 int launch_typed(AttnArgs& a, int D, int group, cudaStream_t st) {
-  const bool one = a.rows <= 8;
-  if (D == 64) {
-    if (a.rows > 16) return launch<T, 64, 64, 4>(a, st);
-    return one ? launch<T, 64, 64, 1>(a, st) : launch<T, 64, 64, 2>(a, st);
-  }
-  if (group == 64) return one ? launch<T, 128, 64, 1>(a, st) : launch<T, 128, 64, 2>(a, st);
-  return one ? launch<T, 128, 128, 1>(a, st) : launch<T, 128, 128, 2>(a, st);
+  if (D == 64) return launch_rows<T, 64, 64>(a, st);
+  return group == 64 ? launch_rows<T, 128, 64>(a, st) : launch_rows<T, 128, 128>(a, st);
 }
 
 }  // namespace
