@@ -425,6 +425,21 @@ def test_cache_attn_rising_scores():
     attn_check(-q, cache, table, lens)
 
 
+def test_cache_attn_many_small_weights():
+    # one key takes half of the weight, 60000 others share the rest at 2^-16 of it each
+    g = gen(29)
+    L, D = 60001, 64
+    cache, table = filled(g, [L], 1, D, 64, 128)
+    t = torch.arange(L, device="cuda")
+    slots = table[0].long()[t // 128] * 128 + t % 128
+    k = torch.zeros(L, 1, D, device="cuda")
+    k[5] = 1.0  # score 11 against 0 with the query below
+    b2.kv_cache_write(cache, k, randn(g, L, 1, D) + 2, slots)
+    q = torch.full((1, 1, 4, D), 11 * D ** 0.5 / D, device="cuda")
+    for dtype in (torch.float16, torch.bfloat16):
+        attn_check(q.to(dtype), cache, table, [L])
+
+
 def test_cache_attn_strides_and_dims():
     g = gen(24)
     lens, Hq, H, D = [40, 70], 4, 2, 64
