@@ -183,6 +183,7 @@ struct KernelArgs {
   void* o;
   long long qt, qh, kt, kh, vt, vh, ot, oh;
   int G, R, Hk, D, causal;
+  unsigned most;  // units that the work list has room for
   float scale_log2;
 };
 
@@ -272,7 +273,8 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     Unit u;
     const unsigned at = r * gridDim.x + ((r & 1) ? (gridDim.x - 1 - blockIdx.x) : blockIdx.x);
     u.valid = at < num_units;
-    if (u.valid) {
+    // loaded without waiting for the number of units: the list has room for a.most
+    if (at < a.most) {
       const unsigned row = at / (unsigned)a.Hk;
       u.kvh = (int)(at - row * a.Hk);
       const int4* p = reinterpret_cast<const int4*>(list + row);
@@ -779,6 +781,7 @@ int launch(const PackedCall& c, cudaStream_t st) {
     set_error("b2_fa_packed: %lld units of work are too many for one launch", most);
     return B2_EINVAL;
   }
+  a.most = (unsigned)most;
   const int sms = device_sm_count();
   // The kernel's prologue (barriers, TMEM, descriptors) runs beside the plan kernel.
   cudaLaunchAttribute attr = {};
