@@ -732,3 +732,117 @@ def test_packed_refusals(bad):
     with pytest.raises(NotImplementedError):
         x = torch.zeros(8, 2, 136, device="cuda").half()
         b2.flash_attn_packed(x, x, x, cu)
+
+
+# ------------------------------------------------------------------ how they are called
+def a_step(g):
+    """Inputs of one decode step and of one prompt call, and the step as a function."""
+    T, Hq, Hk, D = 24, 8, 2, 64
+    q, k, v = randn(g, T, Hq, D).bfloat16(), randn(g, T, Hk, D).bfloat16(), randn(g, T, Hk, D).bfloat16()
+    table, pos = b2.rope_table(64, D), torch.arange(T, device="cuda", dtype=torch.int32)
+    w = (1 + 0.1 * randn(g, D)).bfloat16()
+    cu = torch.tensor([0, 9, T], device="cuda", dtype=torch.int32)
+    cache = b2.kv_cache_alloc(4, Hk, D, 16)
+    slots = torch.arange(T, device="cuda") + 16
+    pages, lengths = torch.tensor([[1, 2]], device="cuda", dtype=torch.int32), torch.tensor([T], device="cuda", dtype=torch.int32)
+
+    def run():
+        qr, kr = b2.qk_norm_rope(q, k, table, pos, w, w)
+        b2.kv_cache_write(cache, kr, v, slots)
+        o = b2.flash_attn_packed(qr, kr, v, cu)
+        o4 = b2.kv_cache_attn(qr[-1:], cache, pages, lengths)
+        return (qr, kr, o, o4, *b2.kv_cache_read(cache, slots, torch.float32))
+    return run, (q, k, v)
+
+
+def test_operators_in_a_cuda_graph():
+    run, (q, k, v) = a_step(gen(40))
+    run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+    g = gen(41)
+    for x in (q, k, v):  # new inputs in the same buffers
+        x.copy_(randn(g, *x.shape))
+    graph.replay()
+    got = [o.clone() for o in outs]
+    assert all(torch.equal(a, b) for a, b in zip(got, run()))
+
+
+def test_operators_repeat_bit_for_bit():
+    run, _ = a_step(gen(42))
+    first = run()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, run()))
+    g = gen(43)  # parts of a sequence are joined in the order of its keys, whichever CTA ends first
+    lens = [5000, 3, 1700]
+    cache, table = filled(g, lens, 2, 128, 64, 16)
+    q, lt = randn(g, 3, 2, 8, 128).half(), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = b2.kv_cache_attn(q, cache, table, lt)
+    assert all(torch.equal(b2.kv_cache_attn(q, cache, table, lt), want) for _ in range(10))
+
+
+def test_operators_on_their_own_streams_and_threads():
+    import threading
+    runs = [a_step(gen(50 + i))[0] for i in range(4)]
+    want = [r() for r in runs]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = runs[i]()
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    failed.append(i)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
+def test_rope_in_place_through_the_c_entry():
+    import ctypes
+    g = gen(44)
+    T, Hq, Hk, D, R = 13, 5, 2, 96, 64
+    q, k = randn(g, T, Hq, D).bfloat16(), randn(g, T, Hk, D).bfloat16()
+    w = (1 + 0.1 * randn(g, D)).bfloat16()
+    table, pos = b2.rope_table(32, R), torch.arange(T, device="cuda", dtype=torch.int64)
+    for inter in (0, 1):
+        want = b2.qk_norm_rope(q, k, table, pos, w, w, interleaved=bool(inter))
+        x, y = q.clone(), k.clone()
+        strides = (ctypes.c_int64 * 8)(Hq * D, D, Hk * D, D, Hq * D, D, Hk * D, D)
+        st = _lib.lib().b2_qk_norm_rope(x.data_ptr(), y.data_ptr(), x.data_ptr(), y.data_ptr(), w.data_ptr(), w.data_ptr(),
+                                        table.data_ptr(), pos.data_ptr(), _lib.B2_I64, T, Hq, Hk, D, R, 32, strides, 1e-6,
+                                        inter, _lib.B2_BF16, torch.cuda.current_stream().cuda_stream)
+        assert st == _lib.B2_OK
+        assert torch.equal(x, want[0]) and torch.equal(y, want[1])
+
+
+def test_cache_attn_needs_its_workspace():
+    import ctypes
+    c = b2.kv_cache_alloc(2, 2, 64, 16)
+    q = torch.zeros(1, 1, 4, 64, device="cuda").half()
+    o, table, lengths = torch.empty_like(q), torch.zeros(1, 2, device="cuda", dtype=torch.int32), torch.ones(1, device="cuda", dtype=torch.int32)
+    shape, strides = (ctypes.c_int64 * 5)(2, 2, 16, 64, 64), (ctypes.c_int64 * 6)(256, 256, 64, 256, 256, 64)
+    args = [x.data_ptr() for x in (q, o, *c, table, lengths)] + [1, 1, 4, 2, 2, shape, strides, 0.1, _lib.B2_F16]
+    stream = torch.cuda.current_stream().cuda_stream
+    need = _lib.lib().b2_query_workspace(4, 1, 2, 2, 64)
+    assert need > 0
+    assert _lib.lib().b2_kv_cache_attn(*args, None, 0, stream) == _lib.B2_EINVAL
+    ws = torch.empty(need + 16, dtype=torch.uint8, device="cuda")
+    assert _lib.lib().b2_kv_cache_attn(*args, ws.data_ptr(), need - 1, stream) == _lib.B2_EINVAL
+    assert _lib.lib().b2_kv_cache_attn(*args, ws.data_ptr() + 8, need, stream) == _lib.B2_EINVAL
+    assert _lib.lib().b2_kv_cache_attn(*args, ws.data_ptr(), need, stream) == _lib.B2_OK
+    assert (o == 0).all()

@@ -254,9 +254,10 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
-  const uint32_t tS[2] = {tmem, tmem + 128};
-  const uint32_t tO[2] = {tmem + 256, tmem + 256 + D};
-  const uint32_t tL[2] = {tmem + 256 + 2 * D, tmem + 256 + 2 * D + 16};  // D <= 64 only
+  // columns of tile t: S_t (and P_t), O_t, and the row sums L_t (D <= 64 only)
+  auto tS = [&](int t) { return tmem + t * 128; };
+  auto tO = [&](int t) { return tmem + 256 + t * D; };
+  auto tL = [&](int t) { return tmem + 256 + 2 * D + t * 16; };
 
   // the work list is the plan kernel's
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -293,7 +294,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (lane == 0) {
       bool ok = true;
       uint32_t g = 0, uq = 0;       // K/V blocks issued, query loads
-      uint32_t tails[2] = {0, 0};   // last blocks issued per V buffer
+      uint32_t tails = 0, tailed = 0;  // bit s: phase of V buffer s's vt_full; used at all
       const uint32_t q_bytes = 2 * C::kAtoms * (uint32_t)(a.G * a.R) * 128;
       Unit next = fetch(0);
       for (uint32_t ui = 0; next.valid && ok; ++ui) {
@@ -325,7 +326,10 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           }
           const bool tail = j == n - 1 && has_tail(u.e, n);
           uint64_t* vbar = tail ? &bars->vt_full[s] : &bars->v_full[s];
-          if (tail) ++tails[s];
+          if (tail) {
+            tails ^= 1u << s;
+            tailed |= 1u << s;
+          }
           mbar_arrive_expect_tx(vbar, C::kTileBytes);
           for (int at = 0; at < C::kAtoms; ++at)
             tma_load_3d(sV + s * C::kTileBytes + at * C::kAtomTileBytes, &tmV, vbar, at * 64, u.kvh,
@@ -345,7 +349,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         drain(&bars->v_full[j & 1], (j >> 1) & 1);
       }
       for (int i = 0; i < 2; ++i)
-        if (tails[i] > 0) drain(&bars->vt_full[i], (tails[i] - 1) & 1);
+        if ((tailed >> i) & 1u) drain(&bars->vt_full[i], ((tails >> i) & 1u) ^ 1u);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA
@@ -365,7 +369,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     (void)dones;
     auto qk = [&](int t, int ks) {
       const uint64_t da = t ? dq1 : dq0, db = ks ? dk1 : dk0;
-      const uint32_t d = t ? tS[1] : tS[0];
+      const uint32_t d = tS(t);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         const uint32_t off16 = ((k / 4) * C::kAtomTileBytes + (k % 4) * 32) >> 4;
@@ -375,20 +379,19 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     };
     auto pv = [&](int t, int vs, bool accumulate) {
       const uint64_t db = vs ? dv1 : dv0;
-      const uint32_t d = t ? tO[1] : tO[0], pa = t ? tS[1] : tS[0];
+      const uint32_t d = tO(t), pa = tS(t);
 #pragma unroll
       for (int k = 0; k < kBN / 16; ++k)
         if (leader) mma_f16_ts(d, pa + k * 8, db + ((k * 16 * 128) >> 4), idO, (k > 0 || accumulate) ? 1u : 0u);
       if constexpr (C::kSumMma) {
 #pragma unroll
         for (int k = 0; k < kBN / 16; ++k)
-          if (leader) mma_f16_ts(tL[t], pa + k * 8, dones, idL, (k > 0 || accumulate) ? 1u : 0u);
+          if (leader) mma_f16_ts(tL(t), pa + k * 8, dones, idL, (k > 0 || accumulate) ? 1u : 0u);
       }
     };
     bool ok = true, issued = false;
     uint32_t g = 0, uq = 0;
-    uint32_t gs[2] = {0, 0};  // P blocks consumed per tile
-    uint32_t co[2] = {0, 0};  // outputs begun per tile
+    uint32_t p_phase = 0, o_phase = 0;  // bit t: phase of tile t's p_full, of its o_empty
     Unit next = fetch(0);
     for (uint32_t ui = 0; next.valid && ok; ++ui) {
       const int n0 = next.e.n0, n1 = next.e.n1, n = max(n0, n1);
@@ -412,35 +415,42 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint32_t gj = g + j, gk = gj + 1;
         const int vs = gj & 1, ks = gk & 1;
         if (!mbar_wait(&bars->v_full[vs], (gj >> 1) & 1, abort_flag, &g_packed_status, DEV_TIMEOUT_TMA)) { ok = false; break; }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int nt = t ? n1 : n0;
-          if (j < nt) {
-            // O_t holds the previous output until its softmax warps have read it
-            if (j == 0) {
-              if (!mbar_wait(&bars->o_empty[t], (co[t] & 1) ^ 1u, abort_flag, &g_packed_status, DEV_TIMEOUT_EPI)) { ok = false; break; }
-              ++co[t];
-            }
-            if (!mbar_wait(&bars->p_full[t], gs[t] & 1, abort_flag, &g_packed_status, DEV_TIMEOUT_EPI)) { ok = false; break; }
-            ++gs[t];
-            tc_fence_after();
-            pv(t, vs, j > 0);
-            if (j == nt - 1 && leader) mma_commit(&bars->o_full[t]);
+        // Both tiles' steps as straight code: a loop over them left their phases in
+        // local memory, read before every P.V.
+        if (j < n0) {
+          // O_t holds the previous output until its softmax warps have read it
+          if (j == 0) {
+            if (!mbar_wait(&bars->o_empty[0], (o_phase & 1u) ^ 1u, abort_flag, &g_packed_status, DEV_TIMEOUT_EPI)) { ok = false; break; }
+            o_phase ^= 1u;
           }
-          if (t == 1 && leader) mma_commit(&bars->v_empty[vs]);
-          if (j + 1 < n) {
-            if (t == 0) {
-              if (!mbar_wait(&bars->k_full[ks], (gk >> 1) & 1, abort_flag, &g_packed_status, DEV_TIMEOUT_TMA)) { ok = false; break; }
-              tc_fence_after();
-            }
-            if (j + 1 < nt) qk(t, ks);
-            if (t == 1) {
-              if (leader) mma_commit(&bars->k_empty[ks]);
-              if (j + 2 == n && leader) mma_commit(&bars->q_empty);  // last Q.K^T of the unit
-            }
-          }
+          if (!mbar_wait(&bars->p_full[0], p_phase & 1u, abort_flag, &g_packed_status, DEV_TIMEOUT_EPI)) { ok = false; break; }
+          p_phase ^= 1u;
+          tc_fence_after();
+          pv(0, vs, j > 0);
+          if (j == n0 - 1 && leader) mma_commit(&bars->o_full[0]);
         }
-        if (!ok) break;
+        if (j + 1 < n) {
+          if (!mbar_wait(&bars->k_full[ks], (gk >> 1) & 1, abort_flag, &g_packed_status, DEV_TIMEOUT_TMA)) { ok = false; break; }
+          tc_fence_after();
+          if (j + 1 < n0) qk(0, ks);
+        }
+        if (j < n1) {
+          if (j == 0) {
+            if (!mbar_wait(&bars->o_empty[1], (o_phase >> 1) ^ 1u, abort_flag, &g_packed_status, DEV_TIMEOUT_EPI)) { ok = false; break; }
+            o_phase ^= 2u;
+          }
+          if (!mbar_wait(&bars->p_full[1], p_phase >> 1, abort_flag, &g_packed_status, DEV_TIMEOUT_EPI)) { ok = false; break; }
+          p_phase ^= 2u;
+          tc_fence_after();
+          pv(1, vs, j > 0);
+          if (j == n1 - 1 && leader) mma_commit(&bars->o_full[1]);
+        }
+        if (leader) mma_commit(&bars->v_empty[vs]);
+        if (j + 1 < n) {
+          if (j + 1 < n1) qk(1, ks);
+          if (leader) mma_commit(&bars->k_empty[ks]);
+          if (j + 2 == n && leader) mma_commit(&bars->q_empty);  // last Q.K^T of the unit
+        }
       }
       g += n;
     }
@@ -455,7 +465,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     // ------------------------------------------- V rows past the sequence's end
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsProducer));
     uint32_t g = 0;
-    uint32_t tails[2] = {0, 0};
+    uint32_t tails = 0;  // bit s: phase of vt_full[s]
     Unit next = fetch(0);
     for (uint32_t ui = 0; next.valid; ++ui) {
       const Unit u = next;
@@ -464,10 +474,10 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       g += n;
       if (n == 0 || !has_tail(u.e, n)) continue;
       const int s = (g - 1) & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars->vt_full[s], tails[s] & 1, abort_flag, &g_packed_status,
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars->vt_full[s], (tails >> s) & 1u, abort_flag, &g_packed_status,
                                              DEV_TIMEOUT_TMA)))
         break;
-      ++tails[s];
+      tails ^= 1u << s;
       const int first = u.e.Lk - (n - 1) * kBN;  // 1 .. 127: rows from here on are not the sequence's
       uint8_t* v = sV + s * C::kTileBytes;
       for (int i = lane; i < (kBN - first) * 8 * C::kAtoms; i += 32) {
@@ -512,7 +522,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         uint32_t sr[kBN];
 #pragma unroll
         for (int c = 0; c < kBN / 32; ++c)
-          tmem_ld32(tS[t] + lane_off + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[c * 32]));
+          tmem_ld32(tS(t) + lane_off + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[c * 32]));
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < kBN; ++e) asm volatile("" : "+r"(sr[e]));
@@ -578,22 +588,22 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           uint32_t r[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) r[e] = p[c * 32 + e];
-          tmem_st32(tS[t] + lane_off + c * 32, r);
+          tmem_st32(tS(t) + lane_off + c * 32, r);
         }
         if (warp_rescale && j > 0) {
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t r[32];
-            tmem_ld32(tO[t] + lane_off + c * 32, r);
+            tmem_ld32(tO(t) + lane_off + c * 32, r);
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
-            tmem_st32(tO[t] + lane_off + c * 32, r);
+            tmem_st32(tO(t) + lane_off + c * 32, r);
           }
           if constexpr (C::kSumMma) {
-            const uint32_t lc = tmem_ld1(tL[t] + lane_off);
+            const uint32_t lc = tmem_ld1(tL(t) + lane_off);
             tmem_ld_wait();
-            tmem_st1(tL[t] + lane_off, __float_as_uint(__uint_as_float(lc) * alpha));
+            tmem_st1(tL(t) + lane_off, __float_as_uint(__uint_as_float(lc) * alpha));
           }
         }
         tmem_st_wait();
@@ -610,7 +620,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         ++co;
         tc_fence_after();
         if constexpr (C::kSumMma) {
-          l_run = __uint_as_float(tmem_ld1(tL[t] + lane_off));
+          l_run = __uint_as_float(tmem_ld1(tL(t) + lane_off));
           tmem_ld_wait();
         }
       }
@@ -621,7 +631,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (n_t > 0) {
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
-          tmem_ld32(tO[t] + lane_off + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+          tmem_ld32(tO(t) + lane_off + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < D; ++e) asm volatile("" : "+r"(r[e]));
