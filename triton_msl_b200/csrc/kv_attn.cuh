@@ -16,7 +16,7 @@ struct AttnArgs {
   long long qb, qn, qh, ob, on, oh, table_stride;
   int B, N, Hq, H, G, page_size, num_pages, max_pages;
   int rows;        // N * G rows share a key head
-  int row_blocks;  // of 4, 8, 16 or 32 rows
+  int row_blocks;  // of 4, 8 or 16 rows
   int page_shift;  // log2(page_size), -1 when it is no power of two
   int q_vec;       // q may be read 16 bytes at a time
   float scale_log2;

@@ -13,7 +13,7 @@
 // Tensor work is mma.sync m16n8k16 with the codes as the A operand, straight from
 // registers: S^T = K.Q^T (16 keys x 8 rows) and O^T = V^T.P^T (16 channels x 8
 // rows). tcgen05 would need the widened codes written to shared or tensor memory
-// first, four times the bytes that came in, and M = 128 rows where 1 to 32 exist.
+// first, four times the bytes that came in, and M = 128 rows where 1 to 16 exist.
 // P^T comes from S^T's registers by one 8x8 transpose (movmatrix). The rows are the
 // (token, head) pairs that share a key head: a key is read once for all of them.
 //
@@ -147,12 +147,16 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 // One row of the group: its token among the new ones and its query head.
 __device__ __forceinline__ int row_token(const AttnArgs& a, int row) { return row / a.G; }
 
+// CTAs per SM that the registers allow.
+template <int D, int NT>
+constexpr int kCtasPerSm = NT == 1 ? 4 : D == 64 ? 3 : 2;
+
 // NT tiles of 8 columns (query rows). COLS = 2: every column is a row, a lane has two of
 // each tile. COLS = 1, for at most 4 rows: rows are the even columns, so that a lane has
 // one live column and the scores, exponentials and weights of the dead one are not
 // computed (half of that work for the common 4 heads on a key head).
 template <typename T, int D, int GROUP, int NT, int COLS>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) kv_attn_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(const __grid_constant__ AttnArgs a) {
   using R = Ring<D, GROUP>;
   constexpr int NG = R::NG, N64 = D / 64, WPT = D / 32, ROWS = COLS * 4 * NT;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -793,7 +797,7 @@ int launch(AttnArgs& a, cudaStream_t st) {
   auto kern = kv_attn_kernel<T, D, GROUP, NT, COLS>;
   static OncePerDevice ready;
   B2_CUDA_TRY(ready([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }));
-  int grid = device_sm_count() * (NT == 1 ? 4 : 2);
+  int grid = device_sm_count() * kCtasPerSm<D, NT>;
   if (grid > kMaxGrid) grid = kMaxGrid;
   kern<<<grid, kThreads, smem, st>>>(a);
   B2_CHECK_LAUNCH();
@@ -814,9 +818,9 @@ template <typename T, int D, int GROUP>
 int launch_rows(AttnArgs& a, cudaStream_t st) {
   if (a.rows <= 4) return launch<T, D, GROUP, 1, 1>(a, st);
   if (a.rows <= 8) return launch<T, D, GROUP, 1, 2>(a, st);
-  if constexpr (D == 64) {  // the registers of D = 128 hold two tiles at most
-    if (a.rows > 16) return launch<T, D, GROUP, 4, 2>(a, st);
-  }
+  // More rows: blocks of 16, each reading the keys again (from L2). Blocks of 32 with
+  // D = 64 (255 registers) measured 62 us against 67 for 16 sequences of up to 32768
+  // keys and 32 rows, but 19.3 against 18.5 up to 4095 and 10.2 against 7.8 up to 64.
   return launch<T, D, GROUP, 2, 2>(a, st);
 }
 
@@ -829,7 +833,7 @@ int launch_typed(AttnArgs& a, int D, int group, cudaStream_t st) {
 }  // namespace
 
 size_t kv_attn_mma_workspace(int64_t rows, int64_t D) {
-  const size_t block = rows <= 8 ? 8 : rows <= 16 || D > 64 ? 16 : 32;
+  const size_t block = rows <= 8 ? 8 : 16;
   return sizeof(float) * 2 * kMaxGrid * block * (size_t)(D + 2);
 }
 
