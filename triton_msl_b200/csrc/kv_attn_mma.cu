@@ -698,7 +698,7 @@ constexpr int kJoinMax = 1024;  // parts whose weights are kept; a segment has a
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kJoin) kv_attn_join_kernel(const __grid_constant__ AttnArgs a, int grid) {
   constexpr int LANES = D / 4, LINES = kJoin / LANES;
-  __shared__ float s_w[kJoinMax], s_top[kJoin / 32], s_total[kJoin / 32];
+  __shared__ float s_w[kJoinMax], s_l[kJoinMax], s_top[kJoin / 32], s_total[kJoin / 32];
   __shared__ float4 s_v[LINES][LANES];
   const int per_seq = a.H * a.rows;
   const int b = blockIdx.x / per_seq, rest = blockIdx.x - b * per_seq;
@@ -727,9 +727,18 @@ __global__ void __launch_bounds__(kJoin) kv_attn_join_kernel(const __grid_consta
   // the first CTA's part began in it (slot 1), the others' began before them (slot 0)
   const size_t stride = (size_t)ROWS * (D + 2);
   auto part = [&](int i) { return a.partials + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * stride; };
-  float top = kNoMax;
+  const int col = threadIdx.x % LANES, first = threadIdx.x / LANES;
+  // Everything a thread can ask for without the weights is asked for first.
+  constexpr int kAhead = 4;
+  float4 ahead[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j)
+    if (first + j * LINES < parts) ahead[j] = *reinterpret_cast<const float4*>(part(first + j * LINES) + r * D + 4 * col);
+  float top = kNoMax, sum = 0.f;
   for (int i = threadIdx.x; i < parts; i += kJoin) {
-    s_w[i] = part(i)[ROWS * D + r];
+    const float* p = part(i) + ROWS * D + r;
+    s_w[i] = p[0];
+    s_l[i] = p[ROWS];
     top = fmaxf(top, s_w[i]);
   }
 #pragma unroll
@@ -738,26 +747,27 @@ __global__ void __launch_bounds__(kJoin) kv_attn_join_kernel(const __grid_consta
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kJoin / 32; ++w) top = fmaxf(top, s_top[w]);
-  float sum = 0.f;
   for (int i = threadIdx.x; i < parts; i += kJoin) {
     s_w[i] = ex2(s_w[i] - top);
-    sum = fmaf(s_w[i], part(i)[ROWS * D + ROWS + r], sum);
+    sum = fmaf(s_w[i], s_l[i], sum);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_total[warp] = sum;
   __syncthreads();
-  const int col = threadIdx.x % LANES, first = threadIdx.x / LANES;
   float4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int i = first; i < parts; i += LINES) {
-    const float4 y = *reinterpret_cast<const float4*>(part(i) + r * D + 4 * col);
-    const float w = s_w[i];
+  auto add = [&](const float4& y, float w) {
     v.x = fmaf(w, y.x, v.x);
     v.y = fmaf(w, y.y, v.y);
     v.z = fmaf(w, y.z, v.z);
     v.w = fmaf(w, y.w, v.w);
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j)
+    if (first + j * LINES < parts) add(ahead[j], s_w[first + j * LINES]);
+#pragma unroll 8
+  for (int i = first + kAhead * LINES; i < parts; i += LINES)
+    add(*reinterpret_cast<const float4*>(part(i) + r * D + 4 * col), s_w[i]);
   s_v[first][col] = v;
   __syncthreads();
   if (first == 0) {
