@@ -18,16 +18,16 @@
 // (token, head) pairs that share a key head: a key is read once for all of them.
 //
 // Work is split along the keys: all sequences' tiles of 128 keys form one line that
-// is cut evenly among the CTAs (four per SM), whatever the lengths. Inside a tile
+// is cut evenly among the CTAs (two to four per SM), whatever the lengths. Inside a tile
 // each of 4 warps takes 32 keys. A warp's codes and scales come by cp.async into its
 // own two buffers of shared memory, so no barrier is needed in the loop. At a
 // sequence's end, or the CTA's, the warps' partial results are merged; a sequence cut
 // between CTAs is joined by kv_attn_join_kernel from partials in the workspace, in the
 // order of the keys.
 //
-// Bound: instructions (half of them widen codes; ALU pipe 54 %, issue slots 58 %) and,
-// on long sequences, HBM. Measured, 32 query heads on 8, D = 128, groups of 64, bf16: 32
-// sequences of up to 8192 tokens 39.8 us, 3.9 TB/s; of up to 32768 126 us, 4.9 TB/s.
+// Bound: instructions (a third of them widen codes; ALU pipe 56 %, issue slots 57 %)
+// and, on long sequences, HBM. Measured, 32 query heads on 8, D = 128, groups of 64,
+// bf16: 32 sequences of up to 8192 tokens 39.2 us, 4.0 TB/s; of up to 32768 126 us, 5.0.
 //
 // Softmax: the running maximum of a row is only raised when a score passes it by 2^8
 // (one vote a step), P = 2^(s - m) then stays below 2^8. P * sv is rounded to fp16
