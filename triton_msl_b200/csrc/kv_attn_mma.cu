@@ -5,10 +5,14 @@
 //   score_rj = sum_g sk_jg (q_r . ck_j)_g + lok_jg (sum of q_r)_g
 //   o_rd     = sum_j (p_rj sv_jg) cv_jd + sum_j p_rj lov_jg
 // so the codes themselves are what is multiplied, and scales and lowest values
-// touch one number per key and group, not one per channel. A 4-bit code in the low
-// mantissa bits of an fp16 is the subnormal c * 2^-24 (or c * 2^-20 four bits up),
-// exactly, so two codes become a tensor-core operand by one AND; the powers of two
-// go into q (a sixteenth for the odd codes) and into the last multiplication.
+// touch one number per key and group, not one per channel. A 4-bit code c0 in the low
+// mantissa bits of an fp16 is the subnormal c0 * 2^-24, exactly, and a byte of two
+// codes is (c0 + 16 c1) * 2^-24. So a word of 8 codes becomes tensor-core operands,
+// for the c0 and for the bytes, by 4 instructions: q0 c0 + q1 c1 =
+// (q0 - q1/16) c0 + q1/16 (c0 + 16 c1), and the values' bytes give sums from which
+// the c0's are taken at the end. (c0 and 16 c1, by a shift and 4 ANDs: 39.2 us
+// where this takes 37.7, 126 where 120.) The powers of two go into the last
+// multiplication.
 //
 // Tensor work is mma.sync m16n8k16 with the codes as the A operand, straight from
 // registers: S^T = K.Q^T (16 keys x 8 rows) and O^T = V^T.P^T (16 channels x 8
@@ -27,7 +31,7 @@
 //
 // Bound: instructions (a third of them widen codes; ALU pipe 56 %, issue slots 57 %)
 // and, on long sequences, HBM. Measured, 32 query heads on 8, D = 128, groups of 64,
-// bf16: 32 sequences of up to 8192 tokens 39.2 us, 4.0 TB/s; of up to 32768 126 us, 5.0.
+// bf16: 32 sequences of up to 8192 tokens 37.7 us, 4.2 TB/s; of up to 32768 120 us, 5.2.
 //
 // Softmax: the running maximum of a row is only raised when a score passes it by 2^8
 // (one vote a step), P = 2^(s - m) then stays below 2^8. P * sv is rounded to fp16
@@ -136,6 +140,10 @@ __device__ __forceinline__ unsigned count_units(const AttnArgs& a, int b, unsign
   }
   if (before) *before = __reduce_add_sync(0xffffffffu, some);
   return __reduce_add_sync(0xffffffffu, all);
+}
+// Bytes 0 and 2, or 1 and 3, of a word as the low bytes of two halves
+__device__ __forceinline__ uint32_t byte_pair(uint32_t x, int odd) {
+  return odd ? __byte_perm(x, 0, 0x4341) : x & 0x00ff00ffu;
 }
 // 3-input maximum
 __device__ __forceinline__ float max3(float x, float y, float z) {
@@ -326,8 +334,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             const int c0 = 8 * ii + 2 * s;
-            qf[nt][ii * N64 + w][s][0] = half2_bits(x[w][c0], x[w][c0 + 4]);
-            qf[nt][ii * N64 + w][s][1] = half2_bits(x[w][c0 + 1] * 0.0625f, x[w][c0 + 5] * 0.0625f);
+            const float y0 = x[w][c0 + 1] * 0.0625f, y4 = x[w][c0 + 5] * 0.0625f;
+            qf[nt][ii * N64 + w][s][0] = half2_bits(x[w][c0] - y0, x[w][c0 + 4] - y4);
+            qf[nt][ii * N64 + w][s][1] = half2_bits(y0, y4);
           }
       // to the lanes that hold the row's scores: columns 2t, 2t + 1
 #pragma unroll
@@ -387,9 +396,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
       for (int w = 0; w < WPT; ++w)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const uint32_t x0 = s ? k0[w] >> 8 : k0[w], x1 = s ? k1[w] >> 8 : k1[w];
-          const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu;
-          const uint32_t a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+          const uint32_t a2 = byte_pair(k0[w], s), a3 = byte_pair(k1[w], s);
+          const uint32_t a0 = (s ? a2 : k0[w]) & 0x000f000fu, a1 = (s ? a3 : k1[w]) & 0x000f000fu;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
             mma16816(acc[NG == 2 ? w % N64 : 0][nt], a0, a1, a2, a3, qf[nt][w][s][0], qf[nt][w][s][1]);
@@ -550,17 +558,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
       for (int w = 0; w < N64; ++w) {  // channels 64w + 8g ..
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // codes 4h .. 4h+3 of each word
-          uint32_t p0 = __byte_perm(vw[0][w], vw[1][w], h ? 0x7632 : 0x5410);
-          uint32_t p1 = __byte_perm(vw[2][w], vw[3][w], h ? 0x7632 : 0x5410);
+          const uint32_t p0 = __byte_perm(vw[0][w], vw[1][w], h ? 0x7632 : 0x5410);
+          const uint32_t p1 = __byte_perm(vw[2][w], vw[3][w], h ? 0x7632 : 0x5410);
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            const uint32_t a0 = p0 & 0x000f000fu, a1 = p0 & 0x00f000f0u;
-            const uint32_t a2 = p1 & 0x000f000fu, a3 = p1 & 0x00f000f0u;
+            const uint32_t a1 = byte_pair(p0, s), a3 = byte_pair(p1, s);
+            const uint32_t a0 = (s ? a1 : p0) & 0x000f000fu, a2 = (s ? a3 : p1) & 0x000f000fu;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               mma16816(o[w * 4 + 2 * h + s][nt], a0, a1, a2, a3, pf[nt][NG == 2 ? w : 0][0], pf[nt][NG == 2 ? w : 0][1]);
-            p0 >>= 8;
-            p1 >>= 8;
           }
         }
       }
@@ -591,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
         for (int i = 0; i < N64 * 4; ++i) {
           const int d = 64 * (i / 4) + 8 * g + 2 * (i % 4);
           const float y = lo[nt][NG == 2 ? i / 4 : 0][c2];
-          const float2 v = {fmaf(o[i][nt][c2] * 16777216.f, down, y), fmaf(o[i][nt][2 + c2] * 1048576.f, down, y)};
+          const float2 v = {fmaf(o[i][nt][c2] * 16777216.f, down, y), fmaf((o[i][nt][2 + c2] - o[i][nt][c2]) * 1048576.f, down, y)};
           *reinterpret_cast<float2*>(s_o + (warp * ROWS + r) * (D + 4) + d) = v;
         }
       }
