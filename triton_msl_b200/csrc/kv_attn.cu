@@ -158,9 +158,7 @@ int kv_cache_attn_launch(const CacheAttnCall& c, cudaStream_t st, const char** k
     }
     a.partials = static_cast<float*>(c.workspace);
     a.q_vec = (reinterpret_cast<uintptr_t>(c.q) & 15) == 0 && a.qb % 8 == 0 && a.qn % 8 == 0 && a.qh % 8 == 0;
-    a.page_shift = -1;
-    for (int i = 4; i < 31; ++i)
-      if ((1 << i) == a.page_size) a.page_shift = i;
+    a.page_div = FastDiv((uint32_t)a.page_size);
     *kernel = "kv_attn_mma";
     return kv_attn_mma_launch(a, (int)s.D, (int)s.group, c.dtype, st);
   }

@@ -5,6 +5,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "decoder.cuh"
+
 namespace b2 {
 
 struct AttnArgs {
@@ -17,7 +19,7 @@ struct AttnArgs {
   int B, N, Hq, H, G, page_size, num_pages, max_pages;
   int rows;        // N * G rows share a key head
   int row_blocks;  // of 4, 8 or 16 rows
-  int page_shift;  // log2(page_size), -1 when it is no power of two
+  FastDiv page_div;  // by page_size
   int q_vec;       // q may be read 16 bytes at a time
   float scale_log2;
   float* partials;

@@ -31,7 +31,7 @@
 //
 // Bound: instructions (a third of them widen codes; ALU pipe 56 %, issue slots 57 %)
 // and, on long sequences, HBM. Measured, 32 query heads on 8, D = 128, groups of 64,
-// bf16: 32 sequences of up to 8192 tokens 37.7 us, 4.2 TB/s; of up to 32768 120 us, 5.2.
+// bf16: 32 sequences of up to 8192 tokens 37.1 us, 4.2 TB/s; of up to 32768 118 us, 5.3.
 //
 // Softmax: the running maximum of a row is only raised when a score passes it by 2^8
 // (one vote a step), P = 2^(s - m) then stays below 2^8. P * sv is rounded to fp16
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int key = tl * kTile + (warp * kSteps + s) * 16;
-      if (key < sg.keys) page[s] = pages[a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size];
+      if (key < sg.keys) page[s] = pages[a.page_div.div(key)];
     }
   };
   auto load = [&](int tl, int stage) {
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
       if (key < sg.keys) {
         const bool bad = (unsigned)page[s] >= (unsigned)a.num_pages;
         wrong |= bad;
-        const uint32_t in_page = a.page_shift >= 0 ? key & (a.page_size - 1) : key % a.page_size;
+        const uint32_t in_page = key - a.page_div.div(key) * a.page_size;
         const size_t row = (size_t)(bad ? 0u : (unsigned)page[s]) * page_rows + in_page;
         const uint8_t* kc = k_src + row * (D / 2);
         const uint8_t* vc = v_src + row * (D / 2);
