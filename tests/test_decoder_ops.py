@@ -111,7 +111,7 @@ def _attn(B=2, N=1, Hq=4, H=2, D=128, group=64, page=16, max_pages=4, scale=0.1,
     (dict(D=80), _lib.B2_EUNSUPPORTED), (dict(scale=math.inf), _lib.B2_EINVAL), (dict(scale=math.nan), _lib.B2_EINVAL),
     (dict(dt=9), _lib.B2_EINVAL), (dict(q=None), _lib.B2_EINVAL), (dict(table=None), _lib.B2_EINVAL),
     (dict(B=1 << 31), _lib.B2_EINVAL), (dict(max_pages=1 << 27), _lib.B2_EINVAL), (dict(B=0), _lib.B2_OK),
-    (dict(N=0), _lib.B2_OK)])
+    (dict(N=0), _lib.B2_OK), (dict(H=1 << 20, Hq=1 << 20, page=1024), _lib.B2_EINVAL)])
 def test_cache_attn_abi(kw, status):
     assert _attn(**kw) == status
 

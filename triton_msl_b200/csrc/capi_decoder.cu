@@ -195,6 +195,10 @@ int b2_kv_cache_attn(const void* q, void* o, const void* k_codes, const void* k_
     set_error("%s: max_pages * page_size must be below 2^31 - 4096", fn);
     return B2_EINVAL;
   }
+  if (c.shape.pages * c.shape.page_size * c.shape.H > UINT_MAX || c.shape.page_size * c.shape.H > UINT_MAX) {
+    set_error("%s: pages * H * page_size must be < 2^32", fn);
+    return B2_EINVAL;
+  }
   const char* kernel = "";
   const int r = kv_cache_attn_launch(c, reinterpret_cast<cudaStream_t>(stream), &kernel);
   if (r == B2_OK) set_last_kernel(kernel);

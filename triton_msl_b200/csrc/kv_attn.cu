@@ -143,10 +143,6 @@ int kv_cache_attn_launch(const CacheAttnCall& c, cudaStream_t st, const char** k
   a.num_pages = (int)s.pages;
   a.max_pages = (int)c.max_pages;
   a.scale_log2 = c.sm_scale * kLog2e;
-  if (s.H * s.page_size >= (1LL << 32)) {
-    set_error("b2_kv_cache_attn: H * page_size must be < 2^32");
-    return B2_EINVAL;
-  }
   B2_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(&a.status), g_kv_attn_status));
   // fp32 queries would lose bits as fp16 operands; a cache without pages has
   // nothing that the other kernel could load in place of a page that is not there

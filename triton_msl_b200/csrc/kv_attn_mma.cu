@@ -31,7 +31,7 @@
 //
 // Bound: instructions (a third of them widen codes; ALU pipe 56 %, issue slots 57 %)
 // and, on long sequences, HBM. Measured, 32 query heads on 8, D = 128, groups of 64,
-// bf16: 32 sequences of up to 8192 tokens 37.1 us, 4.2 TB/s; of up to 32768 118 us, 5.3.
+// bf16: 32 sequences of up to 8192 tokens 36.8 us, 4.3 TB/s; of up to 32768 117 us, 5.3.
 //
 // Softmax: the running maximum of a row is only raised when a score passes it by 2^8
 // (one vote a step), P = 2^(s - m) then stays below 2^8. P * sv is rounded to fp16
@@ -113,7 +113,7 @@ __device__ __forceinline__ int tiles_of(const AttnArgs& a, int b) { return (keys
 // The line of all work: sequence after sequence, in each segment after segment (key
 // head, block of rows), a segment kSetup units for its start and end, then its tiles.
 // CTA c of n holds units [share * c + min(c, more), ...). Measured on 32 sequences of
-// up to 2048 / 8192 keys: kSetup 0: 22.1 / 48.5 us, 1: 19.0 / 45.1, 2: 18.6 / 44.1.
+// up to 2048 / 8192 keys: kSetup 1: 15.7 / 37.7 us, 2: 15.6 / 36.7, 3: 16.6 / 37.7.
 constexpr int kSetup = 2;
 struct Line {
   unsigned share, more, ctas;
@@ -167,6 +167,11 @@ template <typename T, int D, int GROUP, int NT, int COLS>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(const __grid_constant__ AttnArgs a) {
   using R = Ring<D, GROUP>;
   constexpr int NG = R::NG, N64 = D / 64, WPT = D / 32, ROWS = COLS * 4 * NT;
+  // With a column to spare per row, the weights of a row's second group take it: one
+  // operand then serves both groups, whose sums are in columns of their own (118 ->
+  // 117 us for 32 sequences of up to 32768 tokens).
+  constexpr bool kBoth = COLS == 1 && NG == 2;
+  auto column = [](int i, int c2) { return kBoth ? i / 4 : c2; };  // of o[i] and a row
   extern __shared__ __align__(16) uint8_t smem[];
   float* s_o = reinterpret_cast<float*>(smem + kWarps * kStages * kSteps * R::kStage);  // [warp][row][D + 4]
   float* s_m = s_o + kWarps * ROWS * (D + 4);                                  // [warp][row]
@@ -242,16 +247,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
         const bool bad = (unsigned)page[s] >= (unsigned)a.num_pages;
         wrong |= bad;
         const uint32_t in_page = key - a.page_div.div(key) * a.page_size;
-        const size_t row = (size_t)(bad ? 0u : (unsigned)page[s]) * page_rows + in_page;
-        const uint8_t* kc = k_src + row * (D / 2);
-        const uint8_t* vc = v_src + row * (D / 2);
+        const uint32_t row = (bad ? 0u : (unsigned)page[s]) * page_rows + in_page;  // the cache has < 2^32
+        const uint8_t* kc = k_src + (uint64_t)row * (D / 2);
+        const uint8_t* vc = v_src + (uint64_t)row * (D / 2);
         const uint32_t dst = ring_addr + (stage * kSteps + s) * R::kStage;
 #pragma unroll
         for (int i = 0; i < R::kCodes / 512; ++i) {
           cp_async16(dst + lane * 16 + i * 512, kc + i * 512);
           cp_async16(dst + v_dst + i * 512, vc + i * 512);  // 8 rows further: the same place, 512 bytes on
         }
-        if (s_lane) cp_async16(dst + s_dst, s_src + row * (NG * 4));
+        if (s_lane) cp_async16(dst + s_dst, s_src + (uint64_t)row * (NG * 4));
       }
     }
     cp_async_commit();
@@ -486,8 +491,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
           for (int k = 0; k < NG; ++k) lo[nt][k][c2] *= al;
 #pragma unroll
           for (int i = 0; i < N64 * 4; ++i) {
-            o[i][nt][c2] *= al * ratio;
-            o[i][nt][2 + c2] *= al * ratio;
+            o[i][nt][column(i, c2)] *= al * ratio;
+            o[i][nt][2 + column(i, c2)] *= al * ratio;
           }
         }
       fresh = false;
@@ -497,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
 #pragma unroll
     for (int u = 0; u < kSteps; ++u) {
       // weights, and their products with the values' scales as the B operand
-      uint32_t pf[NT][NG][2];
+      uint32_t pf[NT][kBoth ? 1 : NG][2];
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         sv[u][0][k] *= F;
@@ -505,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float p[4];
+        float p[4], both[NG][2];
 #pragma unroll
         for (int i = 0; i < 4; i += 3 - COLS) {
           p[i] = ex2(x[u][nt][i]);
@@ -528,6 +533,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
 #pragma unroll
             for (int i = 0; i < 4; i += 3 - COLS) lo[nt][k][i & 1] = fmaf(p[i], lv[u][i >> 1][k], lo[nt][k][i & 1]);
           }
+          if constexpr (kBoth) {
+            both[k][0] = w[0];
+            both[k][1] = w[2];
+            if (k == 0) continue;
+            w[1] = w[0], w[3] = w[2];
+            w[0] = both[0][0], w[2] = both[0][1];
+          }
           uint32_t packed[2] = {half2_bits(w[0], w[1]), half2_bits(w[2], w[3])};
           if constexpr (std::is_same<T, __half>::value) {
             // What the rounding took from a weight, times the middle of the codes, goes
@@ -538,12 +550,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&packed[h]));
-              lo[nt][k][0] = fmaf(w[2 * h] - r.x, mid, lo[nt][k][0]);
+              lo[nt][kBoth ? 0 : k][0] = fmaf(w[2 * h] - r.x, mid, lo[nt][kBoth ? 0 : k][0]);
+              if constexpr (kBoth) lo[nt][1][0] = fmaf(w[2 * h + 1] - r.y, mid, lo[nt][1][0]);
               if constexpr (COLS == 2) lo[nt][k][1] = fmaf(w[2 * h + 1] - r.y, mid, lo[nt][k][1]);
             }
           }
-          pf[nt][k][0] = transpose8(packed[0]);
-          pf[nt][k][1] = transpose8(packed[1]);
+          pf[nt][kBoth ? 0 : k][0] = transpose8(packed[0]);
+          pf[nt][kBoth ? 0 : k][1] = transpose8(packed[1]);
         }
       }
       // values
@@ -566,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
             const uint32_t a0 = (s ? a1 : p0) & 0x000f000fu, a2 = (s ? a3 : p1) & 0x000f000fu;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816(o[w * 4 + 2 * h + s][nt], a0, a1, a2, a3, pf[nt][NG == 2 ? w : 0][0], pf[nt][NG == 2 ? w : 0][1]);
+              mma16816(o[w * 4 + 2 * h + s][nt], a0, a1, a2, a3, pf[nt][kBoth || NG == 1 ? 0 : w][0], pf[nt][kBoth || NG == 1 ? 0 : w][1]);
           }
         }
       }
@@ -597,7 +610,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
         for (int i = 0; i < N64 * 4; ++i) {
           const int d = 64 * (i / 4) + 8 * g + 2 * (i % 4);
           const float y = lo[nt][NG == 2 ? i / 4 : 0][c2];
-          const float2 v = {fmaf(o[i][nt][c2] * 16777216.f, down, y), fmaf((o[i][nt][2 + c2] - o[i][nt][c2]) * 1048576.f, down, y)};
+          const int c = column(i, c2);
+          const float2 v = {fmaf(o[i][nt][c] * 16777216.f, down, y), fmaf((o[i][nt][2 + c] - o[i][nt][c]) * 1048576.f, down, y)};
           *reinterpret_cast<float2*>(s_o + (warp * ROWS + r) * (D + 4) + d) = v;
         }
       }
