@@ -77,7 +77,7 @@ def rope_check(q, k, table, pos, qw, kw, eps, inter):
     for got, x, w in ((qo, q, qw), (ko, k, kw)):
         assert got.is_contiguous() and got.dtype == x.dtype
         ref = rope_ref(x, w, table, pos, eps, inter)
-        top = ref.abs().amax(-1, keepdim=True) if ref.numel() else ref
+        top = ref.abs().nan_to_num(0).amax(-1, keepdim=True) if ref.numel() else ref
         check(got, ref, 1e-5 * top, x.dtype)
 
 
@@ -94,6 +94,22 @@ def test_rope(dtype, inter, T, Hq, Hk, D, R, norm):
     table = b2.rope_table(300, R)
     pos = torch.randint(0, 300, (T,), generator=g, device="cuda", dtype=torch.int64 if T % 2 else torch.int32)
     rope_check(q, k, table, pos, qw, kw, 1e-6, inter)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("T,Hq,Hk,D,R,norm", [
+    (1800, 32, 8, 128, 64, True), (3001, 32, 8, 128, 128, True), (4500, 33, 5, 128, 128, True), (9001, 13, 1, 64, 32, False),
+    (9000, 14, 2, 40, 24, True), (1500, 33, 5, 256, 256, True), (9000, 10, 0, 128, 128, True), (18000, 6, 6, 32, 32, False)])
+def test_rope_many_heads_at_a_time(dtype, inter, T, Hq, Hk, D, R, norm):
+    # enough tokens for lane groups of 8, 16 and 32 heads, whole and not; q and k inside one projection
+    g = gen(T + D + R)
+    qkv = randn(g, T, Hq + 2 * Hk, D).mul(2).to(dtype)
+    qkv[T // 2, 1, D - 1] = math.nan  # stays in its head
+    qw, kw = ((1 + 0.3 * randn(g, D)).to(dtype) if norm else None for _ in range(2))
+    table = b2.rope_table(300, R)
+    pos = torch.randint(0, 300, (T,), generator=g, device="cuda", dtype=torch.int64 if T % 2 else torch.int32)
+    rope_check(qkv[:, :Hq], qkv[:, Hq:Hq + Hk], table, pos, qw, kw, 1e-6, inter)
 
 
 @pytest.mark.parametrize("inter", [False, True])

@@ -7,15 +7,16 @@
 //
 // Bound: HBM. Each value is read once and written once; the table row of a
 // token (4R bytes) is shared by its heads and mostly served by the L1 cache.
-// A lane group owns four heads of one token: each lane holds the two vectors
-// whose channels rotate into one another, so the rotation needs no exchange,
-// and the norm one shuffle tree; the lane's table values are loaded once for
-// all four heads, whose loads are issued together before any arithmetic.
+// A lane group owns heads of one token, four at a time: each lane holds the two
+// vectors whose channels rotate into one another, so the rotation needs no
+// exchange, and the norm one shuffle tree; the lane's table values are loaded once
+// for all heads, and four heads' loads are issued together before any arithmetic.
 // 16-bit inputs are bound by instructions as much as by HBM (converting, norm and
 // rotation, 16 a value): vectors of 4 channels, 16 lanes a head of 128, leave
 // registers for 24 warps per SM. Measured on 16384 tokens, 32 + 8 heads of 128, norm,
 // half layout: bf16 74 us, 4.7 TB/s (vectors of 8, 16 warps, and a division per head
 // in the norm: 92); fp32 102 us, 6.6 TB/s.
+#include <algorithm>
 #include <type_traits>
 
 #include "b2_common.cuh"
@@ -30,18 +31,26 @@ using namespace fa;
 
 __device__ uint32_t g_rope_status;
 
-constexpr int kRopeThreads = 256;
-
 template <int BYTES> struct RawVec;
 template <> struct RawVec<16> { using type = uint4; };
 template <> struct RawVec<8> { using type = uint2; };
 template <> struct RawVec<4> { using type = uint32_t; };
 template <> struct RawVec<2> { using type = uint16_t; };
 
-// Heads per lane group, and CTAs per SM below. When they were chosen (the same case),
-// 4 heads and 3 CTAs (80 registers) took 81 us; 2 heads and 4 CTAs 91; 2 and 5 83; 4
-// and 4 (64 registers, spills) 110.
+// Heads of a lane group at once, and CTAs per SM below. When they were chosen (the same
+// case, groups of 4 heads), 4 heads and 3 CTAs (80 registers) took 81 us; 2 heads and 4
+// CTAs 91; 2 and 5 83; 4 and 4 (64 registers, spills) 110.
 constexpr int kHeads = 4;
+// A LOOP kernel's groups take several times 4 heads of a token, the next ones' loads in
+// flight while these are worked on: the angles and addresses, a third of the
+// instructions of 4 heads, are made once for all, and no warp waits for a load it has
+// just asked for. Smaller CTAs end the grid more evenly there (56.1 us; 3 of 256 threads
+// 56.9). With 4 heads a group it is 3 to 8 %
+// slower than a kernel without the loop.
+template <bool LOOP>
+constexpr int kThreadsOf = LOOP ? 128 : 256;
+template <bool LOOP>
+constexpr int kCtasOf = LOOP ? 6 : 3;
 
 struct RopeTensor {
   const void* x;
@@ -60,7 +69,8 @@ struct RopeArgs {
   unsigned groups[2];    // lane groups of each tensor
   unsigned items[2];     // of a token
   FastDiv by_items[2];
-  int pos64, D, R, log_tpr, heads_per_group;
+  int pos64, D, R, log_tpr;
+  int heads_per_group[2];  // of each tensor's lane groups; at most kHeads without LOOP
   float eps, inv_dim;
 };
 
@@ -158,21 +168,22 @@ __device__ __forceinline__ void narrow(const float (&a)[VE], const float (&b)[VE
 // rotated: channels [u VE, u VE + VE) with those R/2 above (half layout), or the
 // 2 VE neighbours from 2 u VE (interleaved). The other units are copied.
 // TPR lanes share a head (0: 1 << log_tpr).
-template <typename T, int VE, int NP, int TPR, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads, NP == 1 ? 3 : 1) rope_kernel(const __grid_constant__ RopeArgs a) {
+template <typename T, int VE, int NP, int TPR, bool INTER, bool LOOP>
+__global__ void __launch_bounds__(kThreadsOf<LOOP>, NP == 1 ? kCtasOf<LOOP> : 1) rope_kernel(const __grid_constant__ RopeArgs a) {
   using Raw = typename RawVec<VE * (int)sizeof(T)>::type;
   const int tpr = TPR ? TPR : 1 << a.log_tpr;
   // A CTA has heads of one tensor, so what belongs to the tensor is uniform in it.
   const int which = blockIdx.x >= a.blocks_q ? 1 : 0;
   const RopeTensor& in = a.in[which];
-  const unsigned tid = (blockIdx.x - (which ? a.blocks_q : 0)) * kRopeThreads + threadIdx.x;
+  const unsigned tid = (blockIdx.x - (which ? a.blocks_q : 0)) * kThreadsOf<LOOP> + threadIdx.x;
   const unsigned gid = TPR ? tid / TPR : tid >> a.log_tpr;
   const int lane = threadIdx.x & (tpr - 1);
   // Lanes past the last group stay for the shuffles and load nothing.
   const bool live = gid < a.groups[which];
   const unsigned token = live ? a.by_items[which].div(gid) : 0;
-  const int h0 = live ? (int)(gid - token * a.items[which]) * a.heads_per_group : 0;
-  const int nh = live ? min(a.heads_per_group, in.heads - h0) : 0;
+  const int per = a.heads_per_group[which];
+  const int h0 = live ? (int)(gid - token * a.items[which]) * per : 0;
+  const int nh = live ? min(per, in.heads - h0) : 0;
   const T* x = static_cast<const T*>(in.x) + (long long)token * in.xt + (long long)h0 * in.xh;
   T* y = static_cast<T*>(in.y) + (long long)token * in.yt + (long long)h0 * in.yh;
   // between a group's heads; the host keeps this within 32 bits
@@ -184,20 +195,23 @@ __global__ void __launch_bounds__(kRopeThreads, NP == 1 ? 3 : 1) rope_kernel(con
   auto second = [&](int u) { return INTER || u >= turned ? 2 * u * VE + VE : u * VE + a.R / 2; };
 
   Raw raw[kHeads][NP][2];
+  auto load = [&](int h) {
 #pragma unroll
-  for (int p = 0; p < NP; ++p) {
-    const int u = lane + p * tpr;
-    const T* const x0 = x + first(u);
-    const int gap = second(u) - first(u);
+    for (int p = 0; p < NP; ++p) {
+      const int u = lane + p * tpr;
+      const T* const x0 = x + first(u);
+      const int gap = second(u) - first(u);
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      raw[i][p][0] = raw[i][p][1] = Raw{};
-      if (i < nh && u < units) {
-        raw[i][p][0] = *reinterpret_cast<const Raw*>(x0 + i * xh);
-        raw[i][p][1] = *reinterpret_cast<const Raw*>(x0 + i * xh + gap);
+      for (int i = 0; i < kHeads; ++i) {
+        raw[i][p][0] = raw[i][p][1] = Raw{};
+        if (h + i < nh && u < units) {
+          raw[i][p][0] = *reinterpret_cast<const Raw*>(x0 + i * xh);
+          raw[i][p][1] = *reinterpret_cast<const Raw*>(x0 + i * xh + gap);
+        }
       }
     }
-  }
+  };
+  load(0);
 
   long long pos = 0;
   if (live) pos = a.pos64 ? static_cast<const long long*>(a.positions)[token]
@@ -262,66 +276,73 @@ __global__ void __launch_bounds__(kRopeThreads, NP == 1 ? 3 : 1) rope_kernel(con
     }
   }
 
-  // the pairs' first and second values, each head's
-  float va[kHeads][NP][VE], vb[kHeads][NP][VE];
+  for (int h = 0; h < (LOOP ? per : 1); h += kHeads) {
+    // the pairs' first and second values, each head's
+    float va[kHeads][NP][VE], vb[kHeads][NP][VE];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i)
+    for (int i = 0; i < kHeads; ++i)
 #pragma unroll
-    for (int p = 0; p < NP; ++p) widen<T, VE, INTER>(raw[i][p], va[i][p], vb[i][p]);
-  // 1/rms of each head; the heads' shuffle trees run beside one another
-  float r[kHeads];
+      for (int p = 0; p < NP; ++p) widen<T, VE, INTER>(raw[i][p], va[i][p], vb[i][p]);
+    if (LOOP && h + kHeads < per) {
+      x += (long long)kHeads * xh;
+      load(h + kHeads);
+    }
+    // 1/rms of each head; the heads' shuffle trees run beside one another
+    float r[kHeads];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) r[i] = 1.f;
-  if (w) {  // the whole CTA alike, so every lane takes part
+    for (int i = 0; i < kHeads; ++i) r[i] = 1.f;
+    if (w) {  // the whole CTA alike, so every lane takes part
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      Vals<VE> s2;
-      s2.fill(0.f);
+      for (int i = 0; i < kHeads; ++i) {
+        Vals<VE> s2;
+        s2.fill(0.f);
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        const Vals<VE> ya(va[i][p]), yb(vb[i][p]);
-        s2 = fma(ya, ya, s2);
-        s2 = fma(yb, yb, s2);
+        for (int p = 0; p < NP; ++p) {
+          const Vals<VE> ya(va[i][p]), yb(vb[i][p]);
+          s2 = fma(ya, ya, s2);
+          s2 = fma(yb, yb, s2);
+        }
+        float t[VE];
+        s2.get(t);
+        r[i] = t[0];
+#pragma unroll
+        for (int e = 1; e < VE; ++e) r[i] += t[e];
       }
-      float t[VE];
-      s2.get(t);
-      r[i] = t[0];
 #pragma unroll
-      for (int e = 1; e < VE; ++e) r[i] += t[e];
+      for (int o = 16; o > 0; o >>= 1)
+        if (o < tpr)
+#pragma unroll
+          for (int i = 0; i < kHeads; ++i) r[i] += __shfl_xor_sync(0xffffffffu, r[i], o);
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) r[i] = rsqrtf(fmaf(r[i], a.inv_dim, a.eps));
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      if (o < tpr)
+    for (int p = 0; p < NP; ++p) {
+      const int u = lane + p * tpr;
+      const Vals<VE> kca(ca[p]), ksb(sb[p]), kcb(cb[p]), ksa(sa[p]);
+      T* const y0 = y + first(u);
+      const int gap = second(u) - first(u);
 #pragma unroll
-        for (int i = 0; i < kHeads; ++i) r[i] += __shfl_xor_sync(0xffffffffu, r[i], o);
-#pragma unroll
-    for (int i = 0; i < kHeads; ++i) r[i] = rsqrtf(fmaf(r[i], a.inv_dim, a.eps));
-  }
-#pragma unroll
-  for (int p = 0; p < NP; ++p) {
-    const int u = lane + p * tpr;
-    const Vals<VE> kca(ca[p]), ksb(sb[p]), kcb(cb[p]), ksa(sa[p]);
-    T* const y0 = y + first(u);
-    const int gap = second(u) - first(u);
-#pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      if (!(i < nh && u < units)) continue;
-      const Vals<VE> xa(va[i][p]), xb(vb[i][p]);
-      Vals<VE> scale;
-      scale.fill(r[i]);
-      Vals<VE> ya = mul(xa, kca), yb = mul(xb, kcb);
-      if (u < turned) {  // the others only take the norm: 0 * inf is not 0
-        ya = fma(xb, ksb, ya);
-        yb = fma(xa, ksa, yb);
+      for (int i = 0; i < kHeads; ++i) {
+        if (!(h + i < nh && u < units)) continue;
+        const Vals<VE> xa(va[i][p]), xb(vb[i][p]);
+        Vals<VE> scale;
+        scale.fill(r[i]);
+        Vals<VE> ya = mul(xa, kca), yb = mul(xb, kcb);
+        if (u < turned) {  // the others only take the norm: 0 * inf is not 0
+          ya = fma(xb, ksb, ya);
+          yb = fma(xa, ksa, yb);
+        }
+        float oa[VE], ob[VE];
+        mul(ya, scale).get(oa);
+        mul(yb, scale).get(ob);
+        Raw out[2];
+        narrow<T, VE, INTER>(oa, ob, out);
+        *reinterpret_cast<Raw*>(y0 + i * yh) = out[0];
+        *reinterpret_cast<Raw*>(y0 + i * yh + gap) = out[1];
       }
-      float oa[VE], ob[VE];
-      mul(ya, scale).get(oa);
-      mul(yb, scale).get(ob);
-      Raw out[2];
-      narrow<T, VE, INTER>(oa, ob, out);
-      *reinterpret_cast<Raw*>(y0 + i * yh) = out[0];
-      *reinterpret_cast<Raw*>(y0 + i * yh + gap) = out[1];
     }
+    if (LOOP) y += (long long)kHeads * yh;
   }
 }
 
@@ -331,33 +352,58 @@ int launch(RopeArgs& a, long long tokens, bool inter, cudaStream_t st) {
   const long long far = 1LL << 28;
   const bool near = a.in[0].xh < far && a.in[0].yh < far && a.in[1].xh < far && a.in[1].yh < far &&
                     a.in[0].xh > -far && a.in[0].yh > -far && a.in[1].xh > -far && a.in[1].yh > -far;
-  const int per = near ? kHeads : 1;
   const int units = a.D / (2 * VE);
   a.log_tpr = 0;
   while ((1 << a.log_tpr) < units && a.log_tpr < 5) ++a.log_tpr;
-  a.heads_per_group = per;
+  auto items_of = [&](int i, int per) { return ((long long)a.in[i].heads + per - 1) / per; };
+  int per = near ? kHeads : 1;
+  bool loop = false;
+  if constexpr (sizeof(T) == 2 && VE == 4 && NP == 1) {
+    // As many heads a group, up to 8 times 4, as leave 5/4 of the warps that the GPU
+    // holds at once. With 32 + 8 heads of 128 and 4 / 8 / 16 / 32 heads a group, in us:
+    // 700 tokens 4.1 / 4.4 / 5.6 / 7.9, 2048 8.6 / 7.9 / 8.5 / 10.4, 4096 16.8 / 14.6 /
+    // 13.4 / 15.1, 16384 76 / 61 / 59 / 56. fp32 is at HBM's rate without (102 us; 105).
+    const long long full = (long long)device_sm_count() * kCtasOf<true> * kThreadsOf<true> * 5 / 4;
+    for (int p = kHeads * 8; near && p > kHeads; p /= 2) {
+      if (((tokens * (items_of(0, p) + items_of(1, p))) << a.log_tpr) < full) continue;
+      per = p;
+      loop = true;
+      break;
+    }
+  }
+  const int cta = loop ? kThreadsOf<true> : kThreadsOf<false>;
   unsigned blocks[2];
   for (int i = 0; i < 2; ++i) {
-    a.items[i] = (unsigned)((a.in[i].heads + per - 1) / per);
+    a.heads_per_group[i] = std::max(1, std::min(per, a.in[i].heads));
+    a.items[i] = (unsigned)items_of(i, per);
     const long long groups = tokens * a.items[i], threads = groups << a.log_tpr;
-    if (groups >= (1LL << 31) || threads + kRopeThreads >= (1LL << 32)) {
+    if (groups >= (1LL << 31) || threads + cta >= (1LL << 32)) {
       set_error("b2_qk_norm_rope: %lld tokens x %u lane groups are too many for one launch", tokens, a.items[i]);
       return B2_EINVAL;
     }
     a.groups[i] = (unsigned)groups;
     a.by_items[i] = FastDiv(a.items[i] ? a.items[i] : 1);
-    blocks[i] = (unsigned)((threads + kRopeThreads - 1) / kRopeThreads);
+    blocks[i] = (unsigned)((threads + cta - 1) / cta);
   }
   a.blocks_q = blocks[0];
   const unsigned grid = blocks[0] + blocks[1];
-  auto run = [&](auto kernel) { kernel<<<grid, kRopeThreads, 0, st>>>(a); };
+  auto run = [&](auto kernel) { kernel<<<grid, cta, 0, st>>>(a); };
   // The widths of a head of 64 and of 128 in vectors of four are known to the compiler.
   if constexpr (VE == 4 && NP == 1) {
-    if (a.log_tpr == 4) run(inter ? rope_kernel<T, 4, 1, 16, true> : rope_kernel<T, 4, 1, 16, false>);
-    else if (a.log_tpr == 3) run(inter ? rope_kernel<T, 4, 1, 8, true> : rope_kernel<T, 4, 1, 8, false>);
-    else run(inter ? rope_kernel<T, 4, 1, 0, true> : rope_kernel<T, 4, 1, 0, false>);
+    auto wide = [&](auto LOOP) {
+      constexpr bool L = decltype(LOOP)::value;
+      if (a.log_tpr == 4) run(inter ? rope_kernel<T, 4, 1, 16, true, L> : rope_kernel<T, 4, 1, 16, false, L>);
+      else if (a.log_tpr == 3) run(inter ? rope_kernel<T, 4, 1, 8, true, L> : rope_kernel<T, 4, 1, 8, false, L>);
+      else run(inter ? rope_kernel<T, 4, 1, 0, true, L> : rope_kernel<T, 4, 1, 0, false, L>);
+    };
+    if constexpr (sizeof(T) == 2) {
+      if (loop) wide(std::true_type{});
+      else wide(std::false_type{});
+    } else {
+      wide(std::false_type{});
+    }
   } else {
-    run(inter ? rope_kernel<T, VE, NP, 0, true> : rope_kernel<T, VE, NP, 0, false>);
+    run(inter ? rope_kernel<T, VE, NP, 0, true, false> : rope_kernel<T, VE, NP, 0, false, false>);
   }
   B2_CHECK_LAUNCH();
   return B2_OK;
