@@ -10,9 +10,8 @@
 // codes is (c0 + 16 c1) * 2^-24. So a word of 8 codes becomes tensor-core operands,
 // for the c0 and for the bytes, by 4 instructions: q0 c0 + q1 c1 =
 // (q0 - q1/16) c0 + q1/16 (c0 + 16 c1), and the values' bytes give sums from which
-// the c0's are taken at the end. (c0 and 16 c1, by a shift and 4 ANDs: 39.2 us
-// where this takes 37.7, 126 where 120.) The powers of two go into the last
-// multiplication.
+// the c0's are taken at the end (5 by taking c0 and 16 c1: 39.2 us where this
+// takes 37.7, 126 where 120). The powers of two go into the last multiplication.
 //
 // Tensor work is mma.sync m16n8k16 with the codes as the A operand, straight from
 // registers: S^T = K.Q^T (16 keys x 8 rows) and O^T = V^T.P^T (16 channels x 8
@@ -167,6 +166,11 @@ template <typename T, int D, int GROUP, int NT, int COLS>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(const __grid_constant__ AttnArgs a) {
   using R = Ring<D, GROUP>;
   constexpr int NG = R::NG, N64 = D / 64, WPT = D / 32, ROWS = COLS * 4 * NT;
+  // Keys' codes in bytes. The difference q0 - q1/16 is rounded to fp16: 2^-12 of it counts
+  // for nothing beside a bf16 result, but doubled the error of an fp16 one (relative
+  // 2.8e-4 -> 3.9e-4, 2.1e-4 of it the output's rounding), so fp16 keeps q0 and q1/16,
+  // both exact, with c0 and 16 c1.
+  constexpr bool kBytes = std::is_same<T, __nv_bfloat16>::value;
   // With a column to spare per row, the weights of a row's second group take it: one
   // operand then serves both groups, whose sums are in columns of their own (118 ->
   // 117 us for 32 sequences of up to 32768 tokens).
@@ -340,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
           for (int s = 0; s < 2; ++s) {
             const int c0 = 8 * ii + 2 * s;
             const float y0 = x[w][c0 + 1] * 0.0625f, y4 = x[w][c0 + 5] * 0.0625f;
-            qf[nt][ii * N64 + w][s][0] = half2_bits(x[w][c0] - y0, x[w][c0 + 4] - y4);
+            qf[nt][ii * N64 + w][s][0] = kBytes ? half2_bits(x[w][c0] - y0, x[w][c0 + 4] - y4) : half2_bits(x[w][c0], x[w][c0 + 4]);
             qf[nt][ii * N64 + w][s][1] = half2_bits(y0, y4);
           }
       // to the lanes that hold the row's scores: columns 2t, 2t + 1
@@ -401,8 +405,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
       for (int w = 0; w < WPT; ++w)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const uint32_t a2 = byte_pair(k0[w], s), a3 = byte_pair(k1[w], s);
-          const uint32_t a0 = (s ? a2 : k0[w]) & 0x000f000fu, a1 = (s ? a3 : k1[w]) & 0x000f000fu;
+          const uint32_t x0 = s ? byte_pair(k0[w], 1) : k0[w], x1 = s ? byte_pair(k1[w], 1) : k1[w];
+          const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu;
+          const uint32_t a2 = kBytes ? byte_pair(k0[w], s) : x0 & 0x00f000f0u;
+          const uint32_t a3 = kBytes ? byte_pair(k1[w], s) : x1 & 0x00f000f0u;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
             mma16816(acc[NG == 2 ? w % N64 : 0][nt], a0, a1, a2, a3, qf[nt][w][s][0], qf[nt][w][s][1]);
