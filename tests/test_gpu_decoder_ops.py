@@ -409,6 +409,24 @@ def test_cache_attn_many_sequences():
     attn_check(randn(g, len(lens), 1, 2, 64).half(), cache, table, lens)
 
 
+@pytest.mark.parametrize("D,group,Hq", [(64, 64, 16), (128, 64, 16), (128, 128, 96)])
+def test_cache_attn_sums_are_not_shifted(D, group, Hq):
+    # results far smaller than the values they are sums of, weights far apart: what rounds the products must not shift
+    # their sum. Independent errors of 4e-4 (weights and result rounded to fp16) average out over
+    # H * D channels, at 6 sigma; a shift may reach 2^-21 of the values.
+    g = gen(23 + D + Hq)
+    L, H = 30000, 16
+    cache, table = filled(g, [L], H, D, group, 64, extra=0)
+    t = torch.arange(L, device="cuda")
+    slots = table[0].long()[t // 64] * 64 + t % 64
+    b2.kv_cache_write(cache, randn(g, L, H, D) * 2, randn(g, L, H, D), slots)
+    q = randn(g, 1, 1, Hq, D).half()
+    ref, top = attn_ref(q, cache, table, [L], D ** -0.5)
+    got = b2.kv_cache_attn(q, cache, table, torch.tensor([L], dtype=torch.int32, device="cuda"))
+    shift = (got.double() - ref).mean().abs().item()
+    assert shift <= 2.0**-21 * top.item() + 6 * 4e-4 * ref.square().mean().sqrt().item() / math.sqrt(H * D)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_cache_attn_scales(dtype):
     # large and tiny queries, keys of very different steps, values from 1e-6 to 1e4

@@ -11,7 +11,8 @@
 // for the c0 and for the bytes, by 4 instructions: q0 c0 + q1 c1 =
 // (q0 - q1/16) c0 + q1/16 (c0 + 16 c1), and the values' bytes give sums from which
 // the c0's are taken at the end (5 by taking c0 and 16 c1: 39.2 us where this
-// takes 37.7, 126 where 120). The powers of two go into the last multiplication.
+// takes 37.7, 126 where 120). fp16 takes more for a more exact result (kBytes below).
+// The powers of two go into the last multiplication.
 //
 // Tensor work is mma.sync m16n8k16 with the codes as the A operand, straight from
 // registers: S^T = K.Q^T (16 keys x 8 rows) and O^T = V^T.P^T (16 channels x 8
@@ -28,7 +29,7 @@
 // between CTAs is joined by kv_attn_join_kernel from partials in the workspace, in the
 // order of the keys.
 //
-// Bound: instructions (a third of them widen codes; ALU pipe 56 %, issue slots 57 %)
+// Bound: instructions (a third of them widen codes; ALU pipe 53 %, issue slots 57 %)
 // and, on long sequences, HBM. Measured, 32 query heads on 8, D = 128, groups of 64,
 // bf16: 32 sequences of up to 8192 tokens 36.8 us, 4.3 TB/s; of up to 32768 117 us, 5.3.
 //
@@ -166,11 +167,22 @@ template <typename T, int D, int GROUP, int NT, int COLS>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(const __grid_constant__ AttnArgs a) {
   using R = Ring<D, GROUP>;
   constexpr int NG = R::NG, N64 = D / 64, WPT = D / 32, ROWS = COLS * 4 * NT;
-  // Keys' codes in bytes. The difference q0 - q1/16 is rounded to fp16: 2^-12 of it counts
-  // for nothing beside a bf16 result, but doubled the error of an fp16 one (relative
-  // 2.8e-4 -> 3.9e-4, 2.1e-4 of it the output's rounding), so fp16 keeps q0 and q1/16,
-  // both exact, with c0 and 16 c1.
+  // What bf16 results do not resolve and fp16 ones do (relative error of their output's
+  // rounding 2.1e-4):
+  // - Keys' codes in bytes: the difference q0 - q1/16 is rounded to fp16 (2.8e-4 -> 3.9e-4
+  //   for 16 sequences of up to 4095 tokens). fp16 keeps q0 and q1/16, both exact, with c0
+  //   and 16 c1.
+  // - Values' bytes as subnormals: their products' sums come out low by 2^-18 of their
+  //   size. For fp16 the bytes lie 3 bits higher, where the largest are normal numbers
+  //   (4 sequences of up to 42677 tokens: 3.9e-4 -> 2.4e-4).
+  // - The accumulators are cut, not rounded, at every step: low by 2^-25 of a sum of codes
+  //   for each 16 keys a warp takes. For fp16 the codes' middle is taken from the sums
+  //   after each tile, by the weights' own sum (64 key heads of 30000 tokens: 3.4e-4 ->
+  //   2.9e-4, shift 7e-6 -> 5e-7 of values of 1).
+  // The three cost 32 sequences of up to 8192 tokens 40.4 us for bf16's 36.8, of up to
+  // 32768 130 for 117.
   constexpr bool kBytes = std::is_same<T, __nv_bfloat16>::value;
+  constexpr float kUnit = kBytes ? 16777216.f : 2097152.f;  // of the sums of codes
   // With a column to spare per row, the weights of a row's second group take it: one
   // operand then serves both groups, whose sums are in columns of their own (118 ->
   // 117 us for 32 sequences of up to 32768 tokens).
@@ -505,6 +517,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
     }
     // F is a power of two: 1/F by its exponent
     const float mid = 7.5f * __int_as_float((254 << 23) - __float_as_int(F));
+    float sums[NT][kBoth ? 1 : NG][4] = {};  // of the weights of these keys
 #pragma unroll
     for (int u = 0; u < kSteps; ++u) {
       // weights, and their products with the values' scales as the B operand
@@ -551,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
             // What the rounding took from a weight, times the middle of the codes, goes
             // to the lowest values' sum: the rounding then counts for the code's distance
             // from 7.5 and not for the whole code. fp16 results resolve that (16 sequences
-            // of up to 4095 keys: relative error 4.5e-4 without, 2.8e-4 with, 2.1e-4 of it
+            // of up to 4095 keys: relative error 4.5e-4 without, 2.6e-4 with, 2.1e-4 of it
             // the output's rounding); bf16 ones do not.
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -563,6 +576,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
           }
           pf[nt][kBoth ? 0 : k][0] = transpose8(packed[0]);
           pf[nt][kBoth ? 0 : k][1] = transpose8(packed[1]);
+          if constexpr (!kBytes) {
+            constexpr uint32_t kOnes = 0x3c003c00u;
+            mma16816(sums[nt][kBoth ? 0 : k], kOnes, kOnes, kOnes, kOnes, pf[nt][kBoth ? 0 : k][0], pf[nt][kBoth ? 0 : k][1]);
+          }
         }
       }
       // values
@@ -581,14 +598,39 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
           const uint32_t p1 = __byte_perm(vw[2][w], vw[3][w], h ? 0x7632 : 0x5410);
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            const uint32_t a1 = byte_pair(p0, s), a3 = byte_pair(p1, s);
-            const uint32_t a0 = (s ? a1 : p0) & 0x000f000fu, a2 = (s ? a3 : p1) & 0x000f000fu;
+            uint32_t a0, a1, a2, a3;
+            if constexpr (kBytes) {
+              a1 = byte_pair(p0, s), a3 = byte_pair(p1, s);
+              a0 = (s ? a1 : p0) & 0x000f000fu, a2 = (s ? a3 : p1) & 0x000f000fu;
+            } else {
+              const uint32_t y0 = s ? p0 >> 5 : p0 << 3, y1 = s ? p1 >> 5 : p1 << 3;
+              a0 = y0 & 0x00780078u, a1 = y0 & 0x07f807f8u;
+              a2 = y1 & 0x00780078u, a3 = y1 & 0x07f807f8u;
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               mma16816(o[w * 4 + 2 * h + s][nt], a0, a1, a2, a3, pf[nt][kBoth || NG == 1 ? 0 : w][0], pf[nt][kBoth || NG == 1 ? 0 : w][1]);
           }
         }
       }
+    }
+    if constexpr (!kBytes) {  // 7.5, and 127.5 of a byte, from the sums to the lowest values'
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c2 = 0; c2 < COLS; ++c2) {
+#pragma unroll
+          for (int i = 0; i < N64 * 4; ++i) {
+            const int c = column(i, c2);
+            const float w = sums[nt][kBoth || NG == 1 ? 0 : i / 4][c];
+            o[i][nt][c] = fmaf(w, -7.5f / kUnit, o[i][nt][c]);
+            o[i][nt][2 + c] = fmaf(w, -127.5f / kUnit, o[i][nt][2 + c]);
+          }
+          // all eight lanes of a column have its sum
+#pragma unroll
+          for (int k = 0; k < NG; ++k)
+            lo[nt][k][c2] = fmaf(sums[nt][kBoth ? 0 : k][kBoth ? k : c2], 0.125f * mid, lo[nt][k][c2]);
+        }
     }
   };
 
@@ -617,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
           const int d = 64 * (i / 4) + 8 * g + 2 * (i % 4);
           const float y = lo[nt][NG == 2 ? i / 4 : 0][c2];
           const int c = column(i, c2);
-          const float2 v = {fmaf(o[i][nt][c] * 16777216.f, down, y), fmaf((o[i][nt][2 + c] - o[i][nt][c]) * 1048576.f, down, y)};
+          const float2 v = {fmaf(o[i][nt][c] * kUnit, down, y), fmaf((o[i][nt][2 + c] - o[i][nt][c]) * (kUnit / 16.f), down, y)};
           *reinterpret_cast<float2*>(s_o + (warp * ROWS + r) * (D + 4) + d) = v;
         }
       }

@@ -45,8 +45,7 @@ constexpr int kHeads = 4;
 // flight while these are worked on: the angles and addresses, a third of the
 // instructions of 4 heads, are made once for all, and no warp waits for a load it has
 // just asked for. Smaller CTAs end the grid more evenly there (56.1 us; 3 of 256 threads
-// 56.9). With 4 heads a group it is 3 to 8 %
-// slower than a kernel without the loop.
+// 56.9). With 4 heads a group it is 3 to 8 % slower than a kernel without the loop.
 template <bool LOOP>
 constexpr int kThreadsOf = LOOP ? 128 : 256;
 template <bool LOOP>
