@@ -12,10 +12,10 @@
 // exchange, and the norm one shuffle tree; the lane's table values are loaded once
 // for all heads, and four heads' loads are issued together before any arithmetic.
 // 16-bit inputs are bound by instructions as much as by HBM (converting, norm and
-// rotation, 16 a value): vectors of 4 channels, 16 lanes a head of 128, leave
+// rotation, 14 a value): vectors of 4 channels, 16 lanes a head of 128, leave
 // registers for 24 warps per SM. Measured on 16384 tokens, 32 + 8 heads of 128, norm,
-// half layout: bf16 74 us, 4.7 TB/s (vectors of 8, 16 warps, and a division per head
-// in the norm: 92); fp32 102 us, 6.6 TB/s.
+// half layout: bf16 56 us, 6.1 TB/s (4 heads a group 74; vectors of 8, 16 warps, and a
+// division per head in the norm 92); fp32 102 us, 6.7 TB/s.
 #include <algorithm>
 #include <type_traits>
 
