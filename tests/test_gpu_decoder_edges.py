@@ -1,0 +1,54 @@
+"""Decoder-serving operators at the edges of what their inputs may hold.
+
+The tolerances are those of test_gpu_decoder_ops.py, for the reasons given there, unless a test
+says otherwise.
+"""
+import pytest
+import torch
+
+import triton_msl_b200 as b2
+from test_gpu_decoder_ops import attn_check, filled, gen, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    b2.device_status(0)
+    yield
+    assert b2.device_status(0) == 0, "a kernel left a status bit"
+
+
+def slots_of(table, b, t, page):
+    return table[b].long()[t // page] * page + t % page
+
+
+# ----------------------------------------------------- attention over the cache
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("level", [-100.0, -200.0, -1000.0])
+@pytest.mark.parametrize("Hq,D,group", [(1, 64, 64), (4, 128, 64), (4, 128, 128), (8, 64, 64), (8, 128, 64), (16, 128, 128),
+                                        (24, 64, 64)])
+def test_cache_attn_scores_far_below_zero(dtype, level, Hq, D, group):
+    # 2^score is zero for every key; only the scores' differences count. One key, one warp's part of a
+    # tile and one more, and a sequence that is cut between CTAs
+    g = gen(60 + Hq)
+    lens = [1, 33, 5000]
+    cache, table = filled(g, lens, 1, D, group, 16)
+    for b, n in enumerate(lens):
+        k = -level / D**0.5 + 0.3 * randn(g, n, 1, D)
+        b2.kv_cache_write(cache, k, randn(g, n, 1, D), slots_of(table, b, torch.arange(n, device="cuda"), 16))
+    attn_check(torch.full((3, 1, Hq, D), -1.0, device="cuda").to(dtype), cache, table, lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,N", [(4, 1), (4, 2), (8, 2)])
+@pytest.mark.parametrize("low", [(0, 32), (32, 64), (96, 128), (0, 96), (200, 256)])
+def test_cache_attn_some_keys_far_below_the_others(dtype, Hq, N, low):
+    g = gen(61)
+    D = 128
+    cache, table = filled(g, [256], 1, D, 64, 16)
+    t = torch.arange(256, device="cuda")
+    k = 0.3 * randn(g, 256, 1, D)
+    k[low[0]:low[1]] += 300 / D**0.5
+    b2.kv_cache_write(cache, k, randn(g, 256, 1, D), slots_of(table, 0, t, 16))
+    attn_check(torch.full((1, N, Hq, D), -1.0, device="cuda").to(dtype), cache, table, [256])

@@ -497,7 +497,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
           for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
           // the maximum's step; the first keys may set it below its start of 0
           const float up = fresh ? (y > -INFINITY ? y : 0.f) : fmaxf(y, 0.f);
-          const float al = ex2(-up);
+          // what is summed so far shrinks by the step; before the first keys that is
+          // nothing, and a step far down would make it 0 * inf
+          const float al = fresh ? 1.f : ex2(-up);
           m[nt][c2] += up;
 #pragma unroll
           for (int u = 0; u < kSteps; ++u) {
