@@ -3,11 +3,13 @@
 The tolerances are those of test_gpu_decoder_ops.py, for the reasons given there, unless a test
 says otherwise.
 """
+import math
+
 import pytest
 import torch
 
 import triton_msl_b200 as b2
-from test_gpu_decoder_ops import attn_check, filled, gen, randn
+from test_gpu_decoder_ops import U, attn_check, check, filled, gen, packed_check, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +54,27 @@ def test_cache_attn_some_keys_far_below_the_others(dtype, Hq, N, low):
     k[low[0]:low[1]] += 300 / D**0.5
     b2.kv_cache_write(cache, k, randn(g, 256, 1, D), slots_of(table, 0, t, 16))
     attn_check(torch.full((1, N, Hq, D), -1.0, device="cuda").to(dtype), cache, table, [256])
+
+
+# -------------------------------------------------------------- packed prompts
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_packed_queries_without_a_key_are_zero(dtype, D, value):
+    # causal with more queries than keys: query i keeps the keys j <= i - 171, so queries 0..170 keep none,
+    # whatever the values hold that later queries of the same tile attend
+    g = gen(64)
+    Lq, Lk, none = 300, 129, 171
+    q, k, v = randn(g, Lq, 8, D).to(dtype), randn(g, Lk, 2, D).to(dtype), randn(g, Lk, 2, D).to(dtype)
+    cu_q, cu_k = (torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (Lq, Lk))
+    clean = packed_check(q, k, v, [Lq], [Lk])
+    for at in (0, 5, 128):
+        w = v.clone()
+        w[at, 1] = value
+        got = b2.flash_attn_packed(q, k, w, cu_q, cu_k)
+        assert (got[:none] == 0).all()
+        seen = torch.zeros_like(got, dtype=torch.bool)
+        seen[none + at:, 4:] = True
+        tol = 1e-4 if dtype == torch.float32 else (U[dtype] + 3e-4) * v.abs().max().double().item()
+        check(got[~seen], clean[~seen], 2 * tol, dtype)
+        assert not torch.isfinite(got[seen]).any()

@@ -638,6 +638,12 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->o_empty[t]);
+        // a row without a key in a tile with keys: its weights are 0, which a value that
+        // is not finite turns into NaN
+        if (lim <= 0) {
+#pragma unroll
+          for (int e = 0; e < D; ++e) r[e] = 0u;
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < D; ++e) r[e] = 0u;
