@@ -78,3 +78,30 @@ def test_packed_queries_without_a_key_are_zero(dtype, D, value):
         tol = 1e-4 if dtype == torch.float32 else (U[dtype] + 3e-4) * v.abs().max().double().item()
         check(got[~seen], clean[~seen], 2 * tol, dtype)
         assert not torch.isfinite(got[seen]).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_masked_values_of_any_size_do_not_reach_a_result(dtype, D):
+    # a masked key's weight is 0 and not the smallest normal number, which a value of 1e38 would bring back
+    g = gen(65)
+    n = 300
+    q, k, v = (randn(g, n, h, D).to(dtype) for h in (4, 2, 2))
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    w = v.clone()
+    w[250:] = 1e38
+    assert torch.equal(b2.flash_attn_packed(q, k, w, cu)[:250], b2.flash_attn_packed(q, k, v, cu)[:250])
+    x = [y.transpose(0, 1)[None].repeat_interleave(4 // y.shape[1], 1) for y in (q, k, v, w)]
+    assert torch.equal(b2.flash_attn_fwd(x[0], x[1], x[3], causal=True)[:, :, :250],
+                       b2.flash_attn_fwd(x[0], x[1], x[2], causal=True)[:, :, :250])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_packed_scores_that_are_all_minus_infinity_have_no_softmax(dtype, D):
+    g = gen(66)
+    n = 150
+    q, k, v = (randn(g, n, h, D).abs().to(dtype) for h in (4, 2, 2))
+    k[:70, :, 3] = -math.inf  # queries 0..69 see no other key
+    got = b2.flash_attn_packed(q, k, v, torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+    assert torch.isnan(got[:70]).all() and torch.isfinite(got[70:]).all()

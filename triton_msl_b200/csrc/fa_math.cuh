@@ -48,7 +48,9 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return r;
 }
 
-// 2^x for two lanes on the FMA pipe, x clamped to [-126, 126].
+// 2^x for two lanes on the FMA pipe, x <= 126; 0 from x = -127 down, so that a masked
+// score (-inf) has no weight (2^-126 is a normal bf16, which a value of 1e38 brings back).
+// Between -127 and -126 the result lies below 2^-126 and keeps no relative accuracy.
 // Range reduction: t = x + 1.5*2^23 rounded toward -inf holds floor(x) in the
 // low mantissa bits of t; f = x - floor(x) lies in [0, 1); 2^f comes from a
 // cubic p(f) = 1 + f*(c1 + f*(c2 + f*c3)) whose coefficients are this file's
@@ -58,8 +60,9 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 __device__ __forceinline__ void exp2_poly2(float x0, float x1, float& y0, float& y1) {
   constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
   constexpr float c1 = 0.6954244f, c2 = 0.22630768f, c3 = 0.07826797f;
-  x0 = fmaxf(x0, -126.f);
-  x1 = fmaxf(x1, -126.f);
+  // at -127: f = 0 and p = 1 exactly, whose bits less 127 << 23 are 0
+  x0 = fmaxf(x0, -127.f);
+  x1 = fmaxf(x1, -127.f);
   const f2_t x = f2_pack(x0, x1);
   const f2_t t = f2_add_rm(x, f2_pack(kMagic, kMagic));
   const f2_t xi = f2_add(t, f2_pack(-kMagic, -kMagic));
