@@ -334,8 +334,9 @@ int b2_kv_cache_attn(const void* q, void* o, const void* k_codes, const void* k_
  * Causal: query i of a sequence keeps the keys j <= i + (Lk - Lq). Query head h
  * reads key head h / (Hq / Hk). A query without a key, and a token outside every
  * sequence, gives zeros. Other sequences' keys and masked keys cannot reach a
- * result, whatever they hold. Offsets must ascend within [0, T]; others are
- * clamped and set the status. strides[12] = {t, h, d} of q, k, v, o in elements.
+ * result, whatever they hold. Offsets must ascend within [0, T]; others set the
+ * status and are clamped, where cu_q descends to the end of the sequences before.
+ * strides[12] = {t, h, d} of q, k, v, o in elements.
  * fp16/bf16 with D a multiple of 8, unit channel stride, strides that are
  * multiples of 8 and 16-byte aligned pointers run on the tensor cores given the
  * workspace b2_query_workspace(5, B, Tq, Hq/Hk) reports (16-byte aligned); the

@@ -9,7 +9,8 @@ import pytest
 import torch
 
 import triton_msl_b200 as b2
-from test_gpu_decoder_ops import U, attn_check, check, filled, gen, packed_check, randn
+from test_gpu_decoder_ops import U, attn_check, check, filled, gen, packed_check, packed_ref, randn
+from triton_msl_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +106,20 @@ def test_packed_scores_that_are_all_minus_infinity_have_no_softmax(dtype, D):
     k[:70, :, 3] = -math.inf  # queries 0..69 see no other key
     got = b2.flash_attn_packed(q, k, v, torch.tensor([0, n], dtype=torch.int32, device="cuda"))
     assert torch.isnan(got[:70]).all() and torch.isfinite(got[70:]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cu,clamped", [
+    ([0, 200, 100], [0, 200, 200]), ([0, 200, 100, 250], [0, 200, 200, 250]), ([150, 20, 220], [150, 150, 220]),
+    ([0, 300] * 40, [0, 300] + [300] * 78), ([-5, 100, 400], [0, 100, 300]), ([0, 120, -7, 290, 5], [0, 120, 120, 290, 290]),
+    ([0] * 40 + [300, 10, 20, 300], [0] * 40 + [300] * 4)])
+def test_packed_offsets_that_descend(dtype, cu, clamped):
+    # a sequence begins no earlier than the ones before it end: every token belongs to one, and the work
+    # is bounded by the tokens, whatever the offsets hold
+    g = gen(67)
+    q, k, v = (randn(g, 300, h, 64).to(dtype) for h in (4, 2, 2))
+    keys = [i * 300 // (len(cu) - 1) for i in range(len(cu))]
+    got = b2.flash_attn_packed(q, k, v, *(torch.tensor(x, dtype=torch.int32, device="cuda") for x in (cu, keys)))
+    assert b2.device_status(0) == _lib.STATUS_BAD_INDEX
+    ref, top = packed_ref(q, k, v, clamped, keys, True, 64**-0.5)
+    check(got, ref, 1e-4 if dtype == torch.float32 else (U[dtype] + 3e-4) * top, dtype)

@@ -34,16 +34,25 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) fa_packed_simt_kernel(const __grid_constant__ SimtArgs a) {
   __shared__ float Qs[kRows][kMaxD], Ks[kKeys][kMaxD + 1], Vs[kKeys][kMaxD];
   __shared__ int s_seq, s_blk;
+  __shared__ packed::Span s_span;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // The CTA's sequence and block: 32 sequences at a time, prefix sums of their
-  // block counts. The grid has a CTA for every block that can exist, so the
-  // last ones find none.
+  // The CTA's sequence and block: 32 sequences at a time, where the ones before them
+  // end, prefix sums of their block counts. The grid has a CTA for every block that can
+  // exist, so the last ones find none.
   if (warp == 0) {
-    int left = (int)blockIdx.x, seq = -2, blk = 0;
+    int left = (int)blockIdx.x, seq = -2, blk = 0, before = 0;
+    packed::Span own = {0, 0};
     for (int b0 = -1; b0 <= a.B && seq == -2; b0 += 32) {
       const int b = b0 + lane;
-      int cnt = b <= a.B ? (packed::span_of(a.cu_q, b, a.B, a.Tq).len + kRows - 1) / kRows : 0;
+      packed::Span q = b <= a.B ? packed::span_of(a.cu_q, b, a.B, a.Tq) : packed::Span{0, 0};
+      int end = q.start + q.len;
+      for (int o = 1; o < 32; o <<= 1) end = max(end, __shfl_up_sync(0xffffffffu, end, o));
+      end = max(end, before);
+      const int up = __shfl_up_sync(0xffffffffu, end, 1);
+      q = q.after(lane ? up : before);
+      before = __shfl_sync(0xffffffffu, end, 31);
+      const int cnt = (q.len + kRows - 1) / kRows;
       int inc = cnt;
       for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, inc, o);
@@ -53,6 +62,7 @@ __global__ void __launch_bounds__(kThreads) fa_packed_simt_kernel(const __grid_c
       if (hit) {
         const int w = __ffs(hit) - 1;
         seq = b0 + w;
+        own = {__shfl_sync(0xffffffffu, q.start, w), __shfl_sync(0xffffffffu, q.len, w)};
         blk = left - (__shfl_sync(0xffffffffu, inc, w) - __shfl_sync(0xffffffffu, cnt, w));
       } else {
         left -= __shfl_sync(0xffffffffu, inc, 31);
@@ -61,6 +71,7 @@ __global__ void __launch_bounds__(kThreads) fa_packed_simt_kernel(const __grid_c
     if (lane == 0) {
       s_seq = seq;
       s_blk = blk;
+      s_span = own;
     }
     if (blockIdx.x == 0 && blockIdx.y == 0)
       for (int b = lane; b < a.B; b += 32)
@@ -70,7 +81,7 @@ __global__ void __launch_bounds__(kThreads) fa_packed_simt_kernel(const __grid_c
   __syncthreads();
   const int seq = s_seq;
   if (seq == -2) return;
-  const packed::Span sq = packed::span_of(a.cu_q, seq, a.B, a.Tq);
+  const packed::Span sq = s_span;
   const packed::Span sk = seq < 0 || seq >= a.B ? packed::Span{0, 0} : packed::span_of(a.cu_k, seq, a.B, a.Tk);
   const int head = blockIdx.y, kvh = head / (a.Hq / a.Hk);
   const int i0 = s_blk * kRows, off = sk.len - sq.len;

@@ -104,10 +104,23 @@ __global__ void __launch_bounds__(1024) fa_packed_plan_kernel(const PlanArgs a) 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   asm volatile("griddepcontrol.launch_dependents;");
   if (threadIdx.x < kPlanClasses) hist[threadIdx.x] = 0;
-  __syncthreads();
+  bool bad = false, bad_q = false;
+  for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
+    bad_q |= packed::span_bad(a.cu_q, b, a.Tq);
+    bad |= packed::span_bad(a.cu_k, b, a.Tk);
+  }
+  if (bad || bad_q) atomicOr(&g_packed_status, DEV_BAD_INDEX);
+  // Also the barrier behind hist. With query offsets that descend one warp walks the
+  // sequences in order, since where one begins depends on all before it.
+  const bool in_order = __syncthreads_or(bad_q);
   auto for_entries = [&](auto&& f) {
-    for (int b = warp - 1; b <= a.B; b += warps) {
-      const packed::Span q = packed::span_of(a.cu_q, b, a.B, a.Tq);
+    int end = 0;
+    for (int b = in_order ? (warp == 0 ? -1 : a.B + 1) : warp - 1; b <= a.B; b += in_order ? 1 : warps) {
+      packed::Span q = packed::span_of(a.cu_q, b, a.B, a.Tq);
+      if (in_order) {
+        q = q.after(end);
+        end = q.start + q.len;
+      }
       const packed::Span k = b < 0 || b >= a.B ? packed::Span{0, 0} : packed::span_of(a.cu_k, b, a.B, a.Tk);
       for (int blk = lane; blk * 2 * a.R < q.len; blk += 32) {
         const Entry e = make_entry(a, q, k, blk);
@@ -116,9 +129,6 @@ __global__ void __launch_bounds__(1024) fa_packed_plan_kernel(const PlanArgs a) 
     }
   };
   for_entries([&](const Entry&, int cls) { atomicAdd(&hist[cls], 1); });
-  for (int b = threadIdx.x; b < a.B; b += blockDim.x)
-    if (packed::span_bad(a.cu_q, b, a.Tq) || packed::span_bad(a.cu_k, b, a.Tk))
-      atomicOr(&g_packed_status, DEV_BAD_INDEX);
   __syncthreads();
   // prefix sums of the classes, one per thread of the first eight warps
   int own = 0, inc = 0;
@@ -138,8 +148,8 @@ __global__ void __launch_bounds__(1024) fa_packed_plan_kernel(const PlanArgs a) 
   }
   __syncthreads();
   Entry* list = reinterpret_cast<Entry*>(reinterpret_cast<char*>(a.ws) + kPlanHeader);
-  // Offsets that overlap could name more entries than the workspace holds; the
-  // surplus is dropped (the status bit is set).
+  // The spans cover every token once: at most as many entries as the list has room for,
+  // unless something writes the offsets meanwhile.
   const int room = a.Tq / (2 * a.R) + a.B + 2;
   for_entries([&](const Entry& e, int cls) {
     const int at = atomicAdd(&hist[cls], 1);

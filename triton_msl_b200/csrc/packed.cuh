@@ -9,8 +9,15 @@ namespace packed {
 // sequence, so that no kernel reads out of range whatever the array holds.
 // The pseudo-sequences -1 and B are the tokens before and after the batch's;
 // they have no keys and get zeros.
+// Where offsets descend, spans of the query axis would overlap: a sequence then
+// begins no earlier than the ones before it end (Span::after), so that the spans of
+// -1 .. B always cover every token once and the work is bounded by T and B.
 struct Span {
   int start, len;
+  __device__ __forceinline__ Span after(int end) const {
+    const int s = max(start, end);
+    return {s, max(start + len - s, 0)};
+  }
 };
 __device__ __forceinline__ Span span_of(const int32_t* cu, int b, int B, int T) {
   int s, e;
