@@ -123,3 +123,25 @@ def test_packed_offsets_that_descend(dtype, cu, clamped):
     assert b2.device_status(0) == _lib.STATUS_BAD_INDEX
     ref, top = packed_ref(q, k, v, clamped, keys, True, 64**-0.5)
     check(got, ref, 1e-4 if dtype == torch.float32 else (U[dtype] + 3e-4) * top, dtype)
+
+
+# ------------------------------------------------------------------ how they are called
+def test_the_binding_refuses_tensors_without_storage():
+    # what a transform wraps has no storage: an exception, and not the end of the process
+    from triton_msl_b200 import decoder_ops
+    native = decoder_ops._native()
+    q, k = torch.ones(2, 6, 4, 64, device="cuda").half(), torch.ones(6, 2, 64, device="cuda").half()
+    table, at = b2.rope_table(8, 64), torch.arange(6, device="cuda", dtype=torch.int32)
+    cache = b2.kv_cache_alloc(1, 2, 64, 16)
+    cu, one = torch.tensor([0, 6], device="cuda", dtype=torch.int32), torch.ones(1, 1, device="cuda", dtype=torch.int32)
+    calls = [lambda x: native.flash_attn_packed(x, k, k, cu, cu, True, 0.1),
+             lambda x: native.qk_norm_rope(x, k, table, at, None, None, 1e-6, False)[0],
+             lambda x: native.kv_cache_attn(x[None], *cache, one, one[0], 0.1),
+             lambda x: native.kv_cache_write(*cache, x[:, :2], x[:, :2], at),
+             lambda x: native.kv_cache_read(*cache, at + x.sum().int() * 0, torch.float16)[0]]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="storage"):
+            torch.vmap(call)(q)
+        with pytest.raises(RuntimeError, match="storage"):
+            torch.func.grad(lambda x: call(x).float().sum())(q[0].float().half())
+    assert torch.equal(b2.flash_attn_packed(q[0], k, k, cu), torch.ones_like(q[0]))

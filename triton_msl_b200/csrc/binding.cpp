@@ -56,6 +56,11 @@ std::string shape_of(const at::Tensor& t) {
 }
 const char* dtype_of(const at::Tensor& t) { return c10::toString(t.scalar_type()); }
 
+struct GilReleased {
+  PyThreadState* const state = PyEval_SaveThread();
+  ~GilReleased() { PyEval_RestoreThread(state); }
+};
+
 // The tensors of one call: all on one CUDA device.
 class Call {
  public:
@@ -111,16 +116,19 @@ class Call {
   at::Tensor empty(c10::IntArrayRef size, at::ScalarType type) const {
     return at::Tensor(at::detail::empty_cuda(size, type, c10::Device(c10::kCUDA, (c10::DeviceIndex)device_), std::nullopt));
   }
-  // Runs f(stream) with the device current; a status other than B2_OK raises.
+  // Runs f(stream) with the device current and the GIL released; a status other than
+  // B2_OK raises. f makes the C call and nothing else: a tensor without storage throws
+  // when its pointer is asked for, so the pointers are taken before.
   template <typename F>
   void run(const char* fn, F&& f) const {
     c10::cuda::OptionalCUDAGuard guard;
     if (c10::cuda::current_device() != device_) guard.set_index((c10::DeviceIndex)device_);
     void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device_).stream();
     int status;
-    Py_BEGIN_ALLOW_THREADS
-    status = f(stream);
-    Py_END_ALLOW_THREADS
+    {
+      const GilReleased released;  // taken back also where f throws
+      status = f(stream);
+    }
     if (status == B2_OK) return;
     // the package's own exception, with the library's message
     PyObject* lib = PyImport_ImportModule("triton_msl_b200._lib");
@@ -201,12 +209,14 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const at::Tensor q = Call::unit(q0), k = Call::unit(k0);
     at::Tensor qo = c.empty({T, Hq, D}, q.scalar_type()), ko = c.empty({T, Hk, D}, q.scalar_type());
     const int64_t strides[8] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), Hq * D, D, Hk * D, D};
+    const void* in[4] = {q.const_data_ptr(), k.const_data_ptr(), weights[0] ? weights[0]->const_data_ptr() : nullptr,
+                         weights[1] ? weights[1]->const_data_ptr() : nullptr};
+    void* out[2] = {qo.mutable_data_ptr(), ko.mutable_data_ptr()};
+    const float* angles = static_cast<const float*>(table.const_data_ptr());
+    const void* at = positions.const_data_ptr();
     c.run("b2_qk_norm_rope", [&](void* stream) {
-      return entries.qk_norm_rope(q.const_data_ptr(), k.const_data_ptr(), qo.mutable_data_ptr(), ko.mutable_data_ptr(),
-                                  weights[0] ? weights[0]->const_data_ptr() : nullptr,
-                                  weights[1] ? weights[1]->const_data_ptr() : nullptr,
-                                  static_cast<const float*>(table.const_data_ptr()), positions.const_data_ptr(), pos, T,
-                                  Hq, Hk, D, R, P, strides, eps, interleaved, dt, stream);
+      return entries.qk_norm_rope(in[0], in[1], out[0], out[1], in[2], in[3], angles, at, pos, T, Hq, Hk, D, R, P, strides,
+                                  eps, interleaved, dt, stream);
     });
     return pair(std::move(qo), std::move(ko));
   });
@@ -234,6 +244,11 @@ struct Cache {
   }
   int64_t H() const { return shape[1]; }
   int64_t D() const { return shape[3]; }
+  // The four arrays, to be read.
+  struct Arrays {
+    const void *kc, *ks, *vc, *vs;
+  };
+  Arrays arrays() const { return {kc.const_data_ptr(), ks.const_data_ptr(), vc.const_data_ptr(), vs.const_data_ptr()}; }
 };
 
 // (k_codes, k_scales, v_codes, v_scales, k, v, slots) -> None
@@ -252,10 +267,11 @@ PyObject* kv_cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int sdt = c.index_code(slots, "slots", T, true);
     const at::Tensor k = Call::unit(k0), v = Call::unit(v0);
     const int64_t strides[4] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
+    const void *kp = k.const_data_ptr(), *vp = v.const_data_ptr(), *at = slots.const_data_ptr();
+    void* to[4] = {cache.kc.mutable_data_ptr(), cache.ks.mutable_data_ptr(), cache.vc.mutable_data_ptr(),
+                   cache.vs.mutable_data_ptr()};
     c.run("b2_kv_cache_write", [&](void* stream) {
-      return entries.kv_cache_write(k.const_data_ptr(), v.const_data_ptr(), cache.kc.mutable_data_ptr(),
-                                    cache.ks.mutable_data_ptr(), cache.vc.mutable_data_ptr(), cache.vs.mutable_data_ptr(),
-                                    slots.const_data_ptr(), sdt, T, cache.shape, strides, dt, stream);
+      return entries.kv_cache_write(kp, vp, to[0], to[1], to[2], to[3], at, sdt, T, cache.shape, strides, dt, stream);
     });
     // the cache was written in place: views that autograd or a tracer holds see a new version
     for (const at::Tensor* t : {&cache.kc, &cache.ks, &cache.vc, &cache.vs})
@@ -282,10 +298,11 @@ PyObject* kv_cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int sdt = c.index_code(slots, "slots", T, true);
     at::Tensor k = c.empty({T, H, D}, type), v = c.empty({T, H, D}, type);
     const int64_t strides[4] = {H * D, D, H * D, D};
+    void *kp = k.mutable_data_ptr(), *vp = v.mutable_data_ptr();
+    const Cache::Arrays from = cache.arrays();
+    const void* at = slots.const_data_ptr();
     c.run("b2_kv_cache_read", [&](void* stream) {
-      return entries.kv_cache_read(k.mutable_data_ptr(), v.mutable_data_ptr(), cache.kc.const_data_ptr(),
-                                   cache.ks.const_data_ptr(), cache.vc.const_data_ptr(), cache.vs.const_data_ptr(),
-                                   slots.const_data_ptr(), sdt, T, cache.shape, strides, dt, stream);
+      return entries.kv_cache_read(kp, vp, from.kc, from.ks, from.vc, from.vs, at, sdt, T, cache.shape, strides, dt, stream);
     });
     return pair(std::move(k), std::move(v));
   });
@@ -315,13 +332,15 @@ PyObject* kv_cache_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int64_t strides[6] = {q.stride(0), q.stride(1), q.stride(2), N * Hq * D, Hq * D, D};
     const size_t ws_bytes = entries.query_workspace(4, B, N * (Hq / H), H, D);
     const at::Tensor ws = ws_bytes ? c.empty({(int64_t)ws_bytes}, at::kByte) : at::Tensor();
+    const void* qp = q.const_data_ptr();
+    void *op = o.mutable_data_ptr(), *wp = ws_bytes ? ws.mutable_data_ptr() : nullptr;
+    const Cache::Arrays from = cache.arrays();
+    const int32_t *pp = static_cast<const int32_t*>(pages.const_data_ptr()),
+                  *lp = static_cast<const int32_t*>(lengths.const_data_ptr());
+    const int64_t max_pages = pages.size(1), table_stride = pages.stride(0);
     c.run("b2_kv_cache_attn", [&](void* stream) {
-      return entries.kv_cache_attn(q.const_data_ptr(), o.mutable_data_ptr(), cache.kc.const_data_ptr(),
-                                   cache.ks.const_data_ptr(), cache.vc.const_data_ptr(), cache.vs.const_data_ptr(),
-                                   static_cast<const int32_t*>(pages.const_data_ptr()),
-                                   static_cast<const int32_t*>(lengths.const_data_ptr()), B, N, Hq, pages.size(1),
-                                   pages.stride(0), cache.shape, strides, scale, dt,
-                                   ws_bytes ? ws.mutable_data_ptr() : nullptr, ws_bytes, stream);
+      return entries.kv_cache_attn(qp, op, from.kc, from.ks, from.vc, from.vs, pp, lp, B, N, Hq, max_pages, table_stride,
+                                   cache.shape, strides, scale, dt, wp, ws_bytes, stream);
     });
     return THPVariable_Wrap(std::move(o));
   });
@@ -351,11 +370,13 @@ PyObject* flash_attn_packed(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
                                  v.stride(0), v.stride(1), v.stride(2), Hq * D,      D,           1};
     const size_t ws_bytes = entries.query_workspace(5, B, Tq, Hq / Hk, 0);
     const at::Tensor ws = ws_bytes ? c.empty({(int64_t)ws_bytes}, at::kByte) : at::Tensor();
+    const void *qp = q.const_data_ptr(), *kp = k.const_data_ptr(), *vp = v.const_data_ptr();
+    void *op = o.mutable_data_ptr(), *wp = ws_bytes ? ws.mutable_data_ptr() : nullptr;
+    const int32_t *cq = static_cast<const int32_t*>(cu_q.const_data_ptr()),
+                  *ck = static_cast<const int32_t*>(cu_k.const_data_ptr());
     c.run("b2_fa_packed", [&](void* stream) {
-      return entries.fa_packed(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(),
-                               static_cast<const int32_t*>(cu_q.const_data_ptr()),
-                               static_cast<const int32_t*>(cu_k.const_data_ptr()), B, Tq, Tk, Hq, Hk, D, strides, scale,
-                               causal, dt, ws_bytes ? ws.mutable_data_ptr() : nullptr, ws_bytes, stream);
+      return entries.fa_packed(qp, kp, vp, op, cq, ck, B, Tq, Tk, Hq, Hk, D, strides, scale, causal, dt, wp, ws_bytes,
+                               stream);
     });
     return THPVariable_Wrap(std::move(o));
   });
