@@ -6,6 +6,10 @@
 // Python (ctypes, torch.empty, tensor attributes) a call took 12 to 22 us, of which the
 // launches are 4 to 7. The C entry points come as addresses from the loaded libb2msl.so
 // (bind), so both bindings use one copy of the library.
+//
+// Each operator has two names: its own makes the call, for the kernel that is registered
+// with torch; direct_... does so only where torch's dispatcher would come to that kernel
+// at once, and otherwise returns NotImplemented, upon which the caller goes through it.
 #include <Python.h>
 
 #include <cstdarg>
@@ -14,11 +18,14 @@
 #include <optional>
 #include <string>
 
+#include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/PyInterpreter.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/b2msl.h"
@@ -382,15 +389,59 @@ PyObject* flash_attn_packed(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
   });
 }
 
-// The addresses of the C entry points, in the order of Entries.
+// torch's mode of a default device, which changes the factories of tensors and nothing here.
+PyObject* device_context = nullptr;
+
+// Whether the dispatcher would bring a call with these arguments to the CUDA kernel and
+// do nothing else on the way: no mode or tracer is on, no transform is at work, and the
+// tensors are what they seem. Everything that would see the call has a key that is
+// included for the thread or is the tensor's own, so nothing has to be named.
+bool plain(PyObject* const* args, Py_ssize_t nargs) {
+  using c10::DispatchKey;
+  using c10::DispatchKeySet;
+  using Modes = at::impl::PythonTorchFunctionTLS;
+  if (at::impl::torch_function_mode_enabled())
+    for (int64_t i = 0; i < Modes::stack_len(); ++i)
+      if ((PyObject*)Py_TYPE(Modes::get_stack_at(i)->ptr(getPyInterpreter())) != device_context) return false;
+  constexpr DispatchKeySet always({DispatchKey::BackendSelect, DispatchKey::ADInplaceOrView});
+  if (!(c10::impl::tls_local_dispatch_key_set().included_ - always).empty()) return false;
+  constexpr DispatchKeySet usual(
+      {DispatchKey::CUDA, DispatchKey::ADInplaceOrView, DispatchKey::AutogradCUDA, DispatchKey::AutocastCUDA});
+  constexpr DispatchKeySet on_cuda(c10::BackendComponent::CUDABit);
+  for (Py_ssize_t i = 0; i < nargs; ++i) {
+    PyObject* const a = args[i];
+    if (a == Py_None || PyFloat_Check(a) || PyLong_Check(a)) continue;
+    if (!THPVariable_CheckExact(a)) {
+      if (THPVariable_Check(a)) return false;  // a subclass
+      continue;
+    }
+    if (THPVariable_Unpack(a).key_set() - usual != on_cuda) return false;
+  }
+  return true;
+}
+// F where the dispatcher has nothing to do, else NotImplemented.
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyObject* direct(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  const int is = [&] {
+    PyObject* done = guarded([&]() -> PyObject* { return plain(args, nargs) ? Py_True : Py_False; });
+    return done ? done == Py_True : -1;
+  }();
+  if (is < 0) return nullptr;
+  if (!is) Py_RETURN_NOTIMPLEMENTED;
+  return F(self, args, nargs);
+}
+
+// The addresses of the C entry points, in the order of Entries, and the class of torch's
+// default-device mode.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
     void* at[6];
-    if (nargs != 6) raise(PyExc_TypeError, "bind: 6 addresses wanted");
+    if (nargs != 7) raise(PyExc_TypeError, "bind: 6 addresses and a class wanted");
     for (int i = 0; i < 6; ++i) {
       at[i] = PyLong_AsVoidPtr(args[i]);
       if (!at[i]) raise(PyErr_Occurred() ? nullptr : PyExc_ValueError, "bind: null address");
     }
+    Py_XSETREF(device_context, Py_NewRef(args[6]));
     entries.qk_norm_rope = reinterpret_cast<decltype(entries.qk_norm_rope)>(at[0]);
     entries.kv_cache_write = reinterpret_cast<decltype(entries.kv_cache_write)>(at[1]);
     entries.kv_cache_read = reinterpret_cast<decltype(entries.kv_cache_read)>(at[2]);
@@ -401,10 +452,12 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-#define B2_METHOD(NAME) \
-  { #NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(NAME)), METH_FASTCALL, nullptr }
-PyMethodDef methods[] = {B2_METHOD(bind),          B2_METHOD(qk_norm_rope),  B2_METHOD(kv_cache_write),
-                         B2_METHOD(kv_cache_read), B2_METHOD(kv_cache_attn), B2_METHOD(flash_attn_packed),
+#define B2_METHOD(NAME, F) \
+  { NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr }
+#define B2_OPERATOR(NAME) B2_METHOD(#NAME, NAME), B2_METHOD("direct_" #NAME, direct<NAME>)
+PyMethodDef methods[] = {B2_METHOD("bind", bind),    B2_OPERATOR(qk_norm_rope),
+                         B2_OPERATOR(kv_cache_write), B2_OPERATOR(kv_cache_read),
+                         B2_OPERATOR(kv_cache_attn),  B2_OPERATOR(flash_attn_packed),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decoder", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -17,8 +17,9 @@ it indexes sets ``STATUS_BAD_INDEX`` in ``device_status()``.
 
 A decode step makes each of these calls once per layer on a few tokens, where the
 host's cost is the call's. So their checks and calls are native
-(``csrc/binding.cpp``), and the functions below go there directly where nothing
-traces; the operators registered with torch serve ``torch.compile`` and other tracers.
+(``csrc/binding.cpp``), and the functions below go there directly where torch's
+dispatcher would do nothing else. Under ``torch.compile``, a tracer, a mode or a
+transform, and for tensors of a subclass, they call the operators registered with torch.
 """
 from __future__ import annotations
 
@@ -27,6 +28,7 @@ import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.utils._device import DeviceContext
 
 from . import _lib
 
@@ -44,7 +46,7 @@ def _native():
         lib = _lib.lib()
         module.bind(*(_lib.address(getattr(lib, f)) for f in (
             "b2_qk_norm_rope", "b2_kv_cache_write", "b2_kv_cache_read", "b2_kv_cache_attn", "b2_fa_packed",
-            "b2_query_workspace")))
+            "b2_query_workspace")), DeviceContext)
         _bound = module
     return _bound
 
@@ -64,9 +66,10 @@ def _register(schema: str, fake) -> None:
     torch.library.register_fake(f"b2msl::{name}", fake, lib=_library)
 
 
-def _traced(x: torch.Tensor) -> bool:
-    """Whether a call on x goes through the registered operator."""
-    return type(x) is not torch.Tensor or torch.compiler.is_compiling()
+# Each function below asks the binding's direct_... first, which makes the call where nothing
+# but the operator's kernel would see it and otherwise returns NotImplemented. The two are
+# written out in each: a shared function for it cost 0.15 us of a call.
+_compiling = torch.compiler.is_compiling
 
 
 # ------------------------------------------------------- q/k norm and rotation
@@ -131,8 +134,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, position
     rotated and not normed. q and k may be strided views (parts of one projection);
     the results are contiguous. A position outside the table gives NaN.
     """
-    call = torch.ops.b2msl.qk_norm_rope.default if _traced(q) else (_bound or _native()).qk_norm_rope
-    return call(q, k, table, positions, q_weight, k_weight, eps, interleaved)
+    if type(q) is torch.Tensor and not _compiling():
+        out = (_bound or _native()).direct_qk_norm_rope(q, k, table, positions, q_weight, k_weight, eps, interleaved)
+        if out is not NotImplemented:
+            return out
+    return torch.ops.b2msl.qk_norm_rope.default(q, k, table, positions, q_weight, k_weight, eps, interleaved)
 
 
 # ------------------------------------------------------------- the 4-bit cache
@@ -183,8 +189,11 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torc
 
     slots: int32 or int64, all different; a negative one marks padding and is skipped.
     """
-    call = torch.ops.b2msl.kv_cache_write.default if _traced(k) else (_bound or _native()).kv_cache_write
-    call(*cache, k, v, slots)
+    if type(k) is torch.Tensor and not _compiling():
+        out = (_bound or _native()).direct_kv_cache_write(*cache, k, v, slots)
+        if out is not NotImplemented:
+            return
+    torch.ops.b2msl.kv_cache_write.default(*cache, k, v, slots)
 
 
 def _read_fake(kc, ks, vc, vs, slots, dtype):
@@ -203,8 +212,11 @@ def kv_cache_read(cache: KVCache, slots: torch.Tensor,
     For the part of a prompt that is already cached: its keys and values, packed
     before the new ones, go to ``flash_attn_packed``.
     """
-    call = torch.ops.b2msl.kv_cache_read.default if _traced(slots) else (_bound or _native()).kv_cache_read
-    return call(*cache, slots, dtype)
+    if type(slots) is torch.Tensor and not _compiling():
+        out = (_bound or _native()).direct_kv_cache_read(*cache, slots, dtype)
+        if out is not NotImplemented:
+            return out
+    return torch.ops.b2msl.kv_cache_read.default(*cache, slots, dtype)
 
 
 # ------------------------------------------------------ attention over the cache
@@ -224,10 +236,13 @@ def kv_cache_attn(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, len
     """
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(q.shape[-1])
-    call = torch.ops.b2msl.kv_cache_attn.default if _traced(q) else (_bound or _native()).kv_cache_attn
     if q.dim() == 3:
-        return call(q.unsqueeze(1), *cache, page_table, lengths, sm_scale).squeeze(1)
-    return call(q, *cache, page_table, lengths, sm_scale)
+        return kv_cache_attn(q.unsqueeze(1), cache, page_table, lengths, sm_scale).squeeze(1)
+    if type(q) is torch.Tensor and not _compiling():
+        out = (_bound or _native()).direct_kv_cache_attn(q, *cache, page_table, lengths, sm_scale)
+        if out is not NotImplemented:
+            return out
+    return torch.ops.b2msl.kv_cache_attn.default(q, *cache, page_table, lengths, sm_scale)
 
 
 # ------------------------------------------------------------- packed prompts
@@ -249,5 +264,10 @@ def flash_attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
     """
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(q.shape[-1])
-    call = torch.ops.b2msl.flash_attn_packed.default if _traced(q) else (_bound or _native()).flash_attn_packed
-    return call(q, k, v, cu_q, cu_q if cu_k is None else cu_k, causal, sm_scale)
+    if cu_k is None:
+        cu_k = cu_q
+    if type(q) is torch.Tensor and not _compiling():
+        out = (_bound or _native()).direct_flash_attn_packed(q, k, v, cu_q, cu_k, causal, sm_scale)
+        if out is not NotImplemented:
+            return out
+    return torch.ops.b2msl.flash_attn_packed.default(q, k, v, cu_q, cu_k, causal, sm_scale)
