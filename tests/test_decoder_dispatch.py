@@ -39,7 +39,7 @@ def stand_in():
     def write(kc, ks, vc, vs, k, v, slots):
         ks.copy_(k.detach().sum().expand(ks.shape))
     return types.SimpleNamespace(
-        qk_norm_rope=lambda q, k, table, pos, qw, kw, eps, inter: (q * 2, k * 3),
+        qk_norm_rope=lambda q, k, table, pos, qw, kw, eps, inter: (q * 2 + (0 if qw is None else qw), k * 3),
         kv_cache_write=write,
         kv_cache_read=lambda kc, ks, vc, vs, slots, dtype: (ks.to(dtype).sum() + slots.to(dtype), slots.to(dtype)),
         kv_cache_attn=lambda q, kc, ks, vc, vs, table, lengths, scale: q * lengths.sum(),
@@ -137,3 +137,39 @@ def test_ordinary_calls_go_directly(monkeypatch):
     w = torch.nn.Parameter(torch.ones(64, device="cuda").half(), requires_grad=False)
     b2.qk_norm_rope(*args[:2], torch.ones(8, 64, device="cuda"), args[2], w, w)
     assert calls[-1] == ("direct_qk_norm_rope", True)
+
+
+def gradients(device):
+    q, k, slots = inputs(device, 4)
+    table, cu, at = torch.ones(8, 64, device=device), torch.tensor([0, 6], device=device, dtype=torch.int32), slots.int()
+    cache = b2.KVCache(*(torch.zeros(*s, device=device, dtype=t) for s, t in (
+        ((1, 2, 16, 32), torch.uint8), ((1, 2, 16, 1, 2), torch.bfloat16)) * 2))
+    pages, w = torch.zeros(1, 1, device=device, dtype=torch.int32), torch.ones(64, device=device).half()
+    calls = [lambda q, k, w: b2.qk_norm_rope(q, k, table, at, w, w), lambda q, k, w: b2.flash_attn_packed(q, k, k, cu),
+             lambda q, k, w: b2.kv_cache_attn(q[:1], cache, pages, at[:1])]
+    for i, call in enumerate(calls):
+        for wants in (0, 1, 2)[:(3, 2, 1)[i]]:
+            x = [y.detach().requires_grad_(j == wants) for j, y in enumerate((q, k, w))]
+            out = call(*x)
+            first = out[0] if isinstance(out, tuple) else out
+            assert first.requires_grad
+            with pytest.raises(RuntimeError, match="b2msl::.* forward-only"):
+                first.float().sum().backward()
+            with torch.no_grad():
+                quiet = call(*x)
+            quiet = quiet[0] if isinstance(quiet, tuple) else quiet
+            assert not quiet.requires_grad and torch.equal(quiet, first)
+    # the cache takes values and no gradients
+    b2.kv_cache_write(cache, k.detach().requires_grad_(), k, slots)
+    assert not any(t.requires_grad for t in cache)
+
+
+def test_a_backward_pass_is_refused(monkeypatch):
+    monkeypatch.setattr(decoder_ops, "_bound", stand_in())
+    gradients("cpu")
+
+
+@pytest.mark.gpu
+def test_a_backward_pass_is_refused_on_the_gpu():
+    gradients("cuda")
+    b2.device_status(0)

@@ -20,6 +20,7 @@
 
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -396,7 +397,8 @@ PyObject* device_context = nullptr;
 // do nothing else on the way: no mode or tracer is on, no transform is at work, and the
 // tensors are what they seem. Everything that would see the call has a key that is
 // included for the thread or is the tensor's own, so nothing has to be named.
-bool plain(PyObject* const* args, Py_ssize_t nargs) {
+// `grads`: nor does a result need a gradient.
+bool plain(bool grads, PyObject* const* args, Py_ssize_t nargs) {
   using c10::DispatchKey;
   using c10::DispatchKeySet;
   using Modes = at::impl::PythonTorchFunctionTLS;
@@ -415,15 +417,18 @@ bool plain(PyObject* const* args, Py_ssize_t nargs) {
       if (THPVariable_Check(a)) return false;  // a subclass
       continue;
     }
-    if (THPVariable_Unpack(a).key_set() - usual != on_cuda) return false;
+    const at::Tensor& t = THPVariable_Unpack(a);
+    if (t.key_set() - usual != on_cuda) return false;
+    if (grads && t.requires_grad() && c10::GradMode::is_enabled()) return false;
   }
   return true;
 }
-// F where the dispatcher has nothing to do, else NotImplemented.
-template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+// F where the dispatcher has nothing to do, else NotImplemented. GRADS: F has results of
+// its tensors' values (a write into the cache has none).
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t), bool GRADS>
 PyObject* direct(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   const int is = [&] {
-    PyObject* done = guarded([&]() -> PyObject* { return plain(args, nargs) ? Py_True : Py_False; });
+    PyObject* done = guarded([&]() -> PyObject* { return plain(GRADS, args, nargs) ? Py_True : Py_False; });
     return done ? done == Py_True : -1;
   }();
   if (is < 0) return nullptr;
@@ -454,10 +459,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 #define B2_METHOD(NAME, F) \
   { NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr }
-#define B2_OPERATOR(NAME) B2_METHOD(#NAME, NAME), B2_METHOD("direct_" #NAME, direct<NAME>)
-PyMethodDef methods[] = {B2_METHOD("bind", bind),    B2_OPERATOR(qk_norm_rope),
-                         B2_OPERATOR(kv_cache_write), B2_OPERATOR(kv_cache_read),
-                         B2_OPERATOR(kv_cache_attn),  B2_OPERATOR(flash_attn_packed),
+#define B2_OPERATOR(NAME, GRADS) B2_METHOD(#NAME, NAME), B2_METHOD("direct_" #NAME, (direct<NAME, GRADS>))
+PyMethodDef methods[] = {B2_METHOD("bind", bind),           B2_OPERATOR(qk_norm_rope, true),
+                         B2_OPERATOR(kv_cache_write, false), B2_OPERATOR(kv_cache_read, true),
+                         B2_OPERATOR(kv_cache_attn, true),   B2_OPERATOR(flash_attn_packed, true),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decoder", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

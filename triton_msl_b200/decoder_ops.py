@@ -11,7 +11,8 @@ current stream:
     with grouped heads
 
 They have no counterparts in the reference. They are forward-only, like the
-attention next to them. Index tensors (positions, slots, pages, lengths, offsets)
+attention next to them: a backward pass through one raises. What is written into the
+cache is held there without its gradient. Index tensors (positions, slots, pages, lengths, offsets)
 are read on the device and never copied to the host; one that points outside what
 it indexes sets ``STATUS_BAD_INDEX`` in ``device_status()``.
 
@@ -19,7 +20,7 @@ A decode step makes each of these calls once per layer on a few tokens, where th
 host's cost is the call's. So their checks and calls are native
 (``csrc/binding.cpp``), and the functions below go there directly where torch's
 dispatcher would do nothing else. Under ``torch.compile``, a tracer, a mode or a
-transform, and for tensors of a subclass, they call the operators registered with torch.
+transform, for tensors of a subclass and where a gradient is wanted, they call the operators registered with torch.
 """
 from __future__ import annotations
 
@@ -64,6 +65,12 @@ def _register(schema: str, fake) -> None:
     # the same checks raise the package's "no CPU path" error on CPU tensors
     _library.impl(name, impl, "CPU")
     torch.library.register_fake(f"b2msl::{name}", fake, lib=_library)
+    if "!" in schema:  # changes its arguments and returns nothing
+        return
+
+    def backward(ctx, *grads):
+        raise RuntimeError(f"b2msl::{name} is forward-only: nothing can be differentiated through it")
+    torch.library.register_autograd(f"b2msl::{name}", backward, lib=_library)
 
 
 # Each function below asks the binding's direct_... first, which makes the call where nothing
