@@ -57,6 +57,17 @@ def test_cache_attn_some_keys_far_below_the_others(dtype, Hq, N, low):
     attn_check(torch.full((1, N, Hq, D), -1.0, device="cuda").to(dtype), cache, table, [256])
 
 
+@pytest.mark.parametrize("Hq", [4, 8, 16])
+def test_cache_attn_tiny_queries_of_huge_keys(Hq):
+    # bf16 has fp32's exponents: queries of 2^-118 against keys of 2^118 have scores of about 1
+    g = gen(62)
+    lens, D = [300], 128
+    cache, table = filled(g, lens, 1, D, 64, 16)
+    t = torch.arange(300, device="cuda")
+    b2.kv_cache_write(cache, randn(g, 300, 1, D) * 2.0**118, randn(g, 300, 1, D), slots_of(table, 0, t, 16))
+    attn_check((randn(g, 1, 1, Hq, D) * 2.0**-118).bfloat16(), cache, table, lens)
+
+
 # -------------------------------------------------------------- packed prompts
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("D", [64, 128])

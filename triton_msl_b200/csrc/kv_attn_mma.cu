@@ -331,7 +331,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
         for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[w][i]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = min(max(268 - (int)(__float_as_uint(top) >> 23), 1), 254);
+      // (both powers, up and down, are normal numbers)
+      const int e = min(max(268 - (int)(__float_as_uint(top) >> 23), 1), 253);
       const float up = __int_as_float(e << 23), down = __int_as_float((254 - e) << 23);
       float sum[NG] = {};
 #pragma unroll
