@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import triton_msl_b200 as b2
-from test_gpu_decoder_ops import U, attn_check, check, filled, gen, packed_check, packed_ref, randn
+from test_gpu_decoder_ops import U, attn_check, attn_ref, check, filled, gen, packed_check, packed_ref, randn
 from triton_msl_b200 import _lib
 
 pytestmark = pytest.mark.gpu
@@ -66,6 +66,41 @@ def test_cache_attn_tiny_queries_of_huge_keys(Hq):
     t = torch.arange(300, device="cuda")
     b2.kv_cache_write(cache, randn(g, 300, 1, D) * 2.0**118, randn(g, 300, 1, D), slots_of(table, 0, t, 16))
     attn_check((randn(g, 1, 1, Hq, D) * 2.0**-118).bfloat16(), cache, table, lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,group,N", [(64, 64, 1), (128, 64, 1), (128, 128, 1), (128, 64, 2), (128, 128, 4), (64, 64, 4)])
+@pytest.mark.parametrize("large", [1e4, 1e6])
+def test_cache_attn_large_values_of_small_weight(dtype, D, group, N, large):
+    # In heads 0 and 2 a few tokens with values 1e6 times the others' weigh nothing, one key half of the
+    # sum and the others, 2^-11.5 of it each, the rest: those products have to keep their bits. Heads 1 and
+    # 3 attend the large ones, so no bound that the heads share can serve both.
+    g = gen(63 + D)
+    B, H, L, page = 24, 8, 4097, 64
+    if dtype == torch.float16 and large > 6e4:
+        large = 6e4 / 5  # what a result of fp16 can hold
+    cache, table = filled(g, [L] * B, H, D, group, page, garbage=False)
+    t = torch.arange(L, device="cuda")
+    outlier = (t % 1024 < 128) & (t % 32 == 7)
+    heavy = torch.zeros(L, dtype=torch.bool, device="cuda")
+    heavy[40] = True
+    q = torch.zeros(B, N, 4 * H, D, device="cuda")
+    q[..., 1] = 8 * D**0.5
+    q[:, :, 0::2, 0], q[:, :, 1::2, 0] = -40 * D**0.5, 40 * D**0.5
+    plain = []
+    for b in range(B):
+        k, v = torch.zeros(L, H, D, device="cuda"), randn(g, L, H, D) + 1
+        k[outlier, :, 0] = 1.0
+        k[heavy, :, 1] = 1.0
+        v[outlier] *= large
+        plain.append(v[~outlier].abs().max().item())
+        b2.kv_cache_write(cache, k, v, slots_of(table, b, t, page))
+    q = q.to(dtype)
+    got = b2.kv_cache_attn(q, cache, table, torch.full((B,), L, dtype=torch.int32, device="cuda"))
+    ref, top = attn_ref(q, cache, table, [L] * B, D**-0.5)
+    check(got[:, :, 1::2], ref[:, :, 1::2], 2e-3 * top, dtype)
+    # the outliers' own part: weight e^-40
+    check(got[:, :, 0::2], ref[:, :, 0::2], 2e-3 * max(plain), dtype)
 
 
 # -------------------------------------------------------------- packed prompts

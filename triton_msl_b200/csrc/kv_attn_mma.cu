@@ -33,12 +33,12 @@
 // and, on long sequences, HBM. Measured, 32 query heads on 8, D = 128, groups of 64,
 // bf16: 32 sequences of up to 8192 tokens 36.8 us, 4.3 TB/s; of up to 32768 117 us, 5.3.
 //
-// Softmax: the running maximum of a row is only raised when a score passes it by 2^8
-// (one vote a step), P = 2^(s - m) then stays below 2^8. P * sv is rounded to fp16
-// (the one rounding of weights, 2^-11); F, a power of two per warp, keeps the largest
-// sv * F at 64 to 128, so that the product uses fp16's range: at most 2^15, and a
-// weight of 2^-20 is not yet subnormal. Scores, sums, the lowest values' part and the
-// accumulators are fp32.
+// Softmax: P = 2^(s - m), and P * sv is rounded to fp16 (the one rounding of weights,
+// 2^-11). So m follows the largest product P * sv of a row and not its largest score: it
+// starts 2^7 to 2^8 below the first, and is raised when one passes 2^15.5 (one vote a step). A
+// product of 2^-21 of the largest so far is not yet subnormal, and large values of small
+// weight leave the others their bits. Scores, sums, the lowest values' part and the
+// accumulators are fp32; P itself, at most 2^65.5, only meets those.
 #include <type_traits>
 
 #include "b2_common.cuh"
@@ -53,6 +53,8 @@ constexpr int kSteps = 2;                    // of 16 keys a warp and tile
 constexpr int kTile = 16 * kSteps * kWarps;  // keys
 // Maximum of no scores.
 constexpr float kNoMax = -3e38f;
+// Bounds of log2(P * sv): where a row's m puts the largest, and where m is raised.
+constexpr float kPut = 8.f, kRaise = 15.5f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -282,9 +284,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
   uint32_t qf[NT][WPT][2][2];          // B operands: code word, low or high byte pair, register
   float f[NT][COLS], qs[NT][NG][COLS]; // per column: factor of the code part, scaled sums of q
   int lim[NT][COLS];                   // keys each column's row keeps
-  float m[NT][COLS], l[NT][COLS], lo[NT][NG][COLS];  // running maximum, sums
+  float m[NT][COLS], l[NT][COLS], lo[NT][NG][COLS];  // the scores' reference, sums
   float o[N64 * 4][NT][4];
-  float F = 0.f;
   int keys_all = 0;                    // keys that every row keeps
   bool fresh = true;                   // no key yet
 
@@ -380,7 +381,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[i][nt][k] = 0.f;
     }
-    F = __int_as_float(254 << 23);
     fresh = true;
     keys_all = max(0, c.keys - a.N + 1);
   };
@@ -465,39 +465,37 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
             for (int k = 0; k < NG; ++k) sv[u][h][k] = lv[u][h][k] = 0.f;
         }
     }
-    // raise the maxima, or lower F, where needed
-    float top_sv = 0.f;  // NaN is left aside
+    // raise the references where needed
+    float log_sv[kSteps][2];  // of the larger scale, at least -50: 0.1 too low at most
 #pragma unroll
     for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-      for (int k = 0; k < NG; ++k) top_sv = max3(top_sv, sv[u][0][k], sv[u][1][k]);
-    float over = top_sv * F * 0.0625f;
+      for (int h = 0; h < 2; ++h) {
+        const float y = max3(sv[u][h][0], sv[u][h][NG - 1], 8.9e-16f);  // NaN is left aside, here and below
+        // exponent and first bits of the mantissa, as they lie in the word, behind 2^23
+        log_sv[u][h] = fmaf(__uint_as_float(__byte_perm(__float_as_uint(y), 0x4b000000u, 0x7632)), 0.0078125f, -65663.f);
+      }
+    float over = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        over = max3(over, x[u][nt][0], x[u][nt][2]);
-        if constexpr (COLS == 2) over = max3(over, x[u][nt][1], x[u][nt][3]);
-      }
-    if (__any_sync(0xffffffffu, over > 8.f) || fresh) {
-      const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top_sv));
-      float ratio = 1.f;
-      if (__uint_as_float(top_bits) * F > 128.f) {  // to 64 .. 128
-        const float to = __int_as_float(min(max(260 - (int)(top_bits >> 23), 1), 254) << 23);
-        ratio = to / F;
-        F = to;
-      }
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c2 = 0; c2 < COLS; ++c2)
+          over = max3(over, x[u][nt][c2] + log_sv[u][0], x[u][nt][2 + c2] + log_sv[u][1]);
+    if (__any_sync(0xffffffffu, over > kRaise) || fresh) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c2 = 0; c2 < COLS; ++c2) {
           float y = -INFINITY;
 #pragma unroll
-          for (int u = 0; u < kSteps; ++u) y = max3(y, x[u][nt][c2], x[u][nt][2 + c2]);
+          for (int u = 0; u < kSteps; ++u) y = max3(y, x[u][nt][c2] + log_sv[u][0], x[u][nt][2 + c2] + log_sv[u][1]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
-          // the maximum's step; the first keys may set it below its start of 0
-          const float up = fresh ? (y > -INFINITY ? y : 0.f) : fmaxf(y, 0.f);
+          // the step; the first keys may set m below its start of 0. Whole numbers: what
+          // changes a reference changes the exponents of the products and no bits
+          const float step = ceilf(y - kPut), up = fresh ? (y > -INFINITY ? step : 0.f) : fmaxf(step, 0.f);
           // what is summed so far shrinks by the step; before the first keys that is
           // nothing, and a step far down would make it 0 * inf
           const float al = fresh ? 1.f : ex2(-up);
@@ -512,24 +510,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
           for (int k = 0; k < NG; ++k) lo[nt][k][c2] *= al;
 #pragma unroll
           for (int i = 0; i < N64 * 4; ++i) {
-            o[i][nt][column(i, c2)] *= al * ratio;
-            o[i][nt][2 + column(i, c2)] *= al * ratio;
+            o[i][nt][column(i, c2)] *= al;
+            o[i][nt][2 + column(i, c2)] *= al;
           }
         }
       fresh = false;
     }
-    // F is a power of two: 1/F by its exponent
-    const float mid = 7.5f * __int_as_float((254 << 23) - __float_as_int(F));
     float sums[NT][kBoth ? 1 : NG][4] = {};  // of the weights of these keys
 #pragma unroll
     for (int u = 0; u < kSteps; ++u) {
       // weights, and their products with the values' scales as the B operand
       uint32_t pf[NT][kBoth ? 1 : NG][2];
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        sv[u][0][k] *= F;
-        sv[u][1][k] *= F;
-      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float p[4], both[NG][2];
@@ -572,9 +563,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&packed[h]));
-              lo[nt][kBoth ? 0 : k][0] = fmaf(w[2 * h] - r.x, mid, lo[nt][kBoth ? 0 : k][0]);
-              if constexpr (kBoth) lo[nt][1][0] = fmaf(w[2 * h + 1] - r.y, mid, lo[nt][1][0]);
-              if constexpr (COLS == 2) lo[nt][k][1] = fmaf(w[2 * h + 1] - r.y, mid, lo[nt][k][1]);
+              lo[nt][kBoth ? 0 : k][0] = fmaf(w[2 * h] - r.x, 7.5f, lo[nt][kBoth ? 0 : k][0]);
+              if constexpr (kBoth) lo[nt][1][0] = fmaf(w[2 * h + 1] - r.y, 7.5f, lo[nt][1][0]);
+              if constexpr (COLS == 2) lo[nt][k][1] = fmaf(w[2 * h + 1] - r.y, 7.5f, lo[nt][k][1]);
             }
           }
           pf[nt][kBoth ? 0 : k][0] = transpose8(packed[0]);
@@ -632,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
           // all eight lanes of a column have its sum
 #pragma unroll
           for (int k = 0; k < NG; ++k)
-            lo[nt][k][c2] = fmaf(sums[nt][kBoth ? 0 : k][kBoth ? k : c2], 0.125f * mid, lo[nt][k][c2]);
+            lo[nt][k][c2] = fmaf(sums[nt][kBoth ? 0 : k][kBoth ? k : c2], 0.125f * 7.5f, lo[nt][k][c2]);
         }
     }
   };
@@ -652,17 +643,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
         }
         if (wrong) l[nt][c2] = __int_as_float(0x7fffffff);  // no such page: the rows are undefined
         const int r = COLS == 2 ? nt * 8 + 2 * t + c2 : t;
+        // l is brought to 1 .. 2, by a power of two, and m to the logarithm of the whole
+        // sum: the warps' references follow their own products and may lie far apart
+        const int e = (int)(__float_as_uint(l[nt][c2]) >> 23);
+        const float down = __int_as_float((254 - e) << 23);
         if (g == 0) {
-          s_m[warp * ROWS + r] = l[nt][c2] == 0.f ? kNoMax : m[nt][c2];
-          s_l[warp * ROWS + r] = l[nt][c2];
+          s_m[warp * ROWS + r] = l[nt][c2] == 0.f ? kNoMax : m[nt][c2] + (float)(e - 127);
+          s_l[warp * ROWS + r] = l[nt][c2] * down;
         }
-        const float down = 1.f / F;  // in range; 2^24 / F need not be
 #pragma unroll
         for (int i = 0; i < N64 * 4; ++i) {
           const int d = 64 * (i / 4) + 8 * g + 2 * (i % 4);
           const float y = lo[nt][NG == 2 ? i / 4 : 0][c2];
           const int c = column(i, c2);
-          const float2 v = {fmaf(o[i][nt][c] * kUnit, down, y), fmaf((o[i][nt][2 + c] - o[i][nt][c]) * (kUnit / 16.f), down, y)};
+          const float2 v = {fmaf(o[i][nt][c], kUnit, y) * down, fmaf(o[i][nt][2 + c] - o[i][nt][c], kUnit / 16.f, y) * down};
           *reinterpret_cast<float2*>(s_o + (warp * ROWS + r) * (D + 4) + d) = v;
         }
       }
