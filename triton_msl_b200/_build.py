@@ -5,15 +5,20 @@ the source or a header changed) and linked into ``triton_msl_b200/libb2msl.so``
 with the CUDA runtime linked statically, so the library carries no dependency
 on the toolkit's shared cudart and travels with the source tree.
 ``csrc/binding.cpp``, the native Python binding of the decoder-serving operators,
-is compiled against torch's headers into ``triton_msl_b200/_decoder.so``.
+is compiled against torch's headers into ``triton_msl_b200/_decoder.<python>.<torch>.so``:
+its name holds the versions that its ABI goes by, so that another torch or Python builds
+its own. One build runs at a time, whatever threads and processes ask for it.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import contextlib
+import fcntl
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -22,7 +27,6 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libb2msl.so"
 BINDING_SRC = CSRC / "binding.cpp"
-BINDING = PKG / "_decoder.so"
 INCLUDE = ROOT / "include"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -63,20 +67,34 @@ def _compile(src: Path, obj: Path, verbose: bool) -> tuple[Path, str]:
     return src, r.stdout + r.stderr
 
 
-def build_binding(force: bool = False) -> Path:
-    """Compile the native binding if its source or the C header changed. Returns its path."""
-    newest = max(p.stat().st_mtime for p in (BINDING_SRC, *INCLUDE.glob("*.h")))
-    if BINDING.exists() and not force and BINDING.stat().st_mtime >= newest:
-        return BINDING
-    import sysconfig
+def binding_path() -> Path:
+    """The native binding for this Python and this torch."""
+    import torch
+    return PKG / f"_decoder.{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}.so"
 
+
+@contextlib.contextmanager
+def _alone():
+    """Waits until no other thread or process builds."""
+    BUILD.mkdir(exist_ok=True)
+    with open(BUILD / ".lock", "w") as f:
+        fcntl.flock(f, fcntl.LOCK_EX)
+        yield
+
+
+def _build_binding(force: bool) -> None:
+    """Compile the native binding if its source or the C header changed."""
+    binding = binding_path()
+    newest = max(p.stat().st_mtime for p in (BINDING_SRC, *INCLUDE.glob("*.h")))
+    if binding.exists() and not force and binding.stat().st_mtime >= newest:
+        return
     import torch
     gxx = shutil.which("g++")
     if gxx is None:
         raise RuntimeError("g++ not found; the native binding cannot be built")
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
-    tmp = BINDING.with_suffix(".so.tmp")
+    tmp = binding.with_name(binding.name + ".tmp")
     cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I", str(root / "include"), "-I", str(root / "include/torch/csrc/api/include"),
@@ -85,14 +103,18 @@ def build_binding(force: bool = False) -> Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {BINDING_SRC.name}:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, BINDING)
-    return BINDING
+    os.replace(tmp, binding)
 
 
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> Path:
     """Compile and link libb2msl.so and the native binding if anything changed. Returns
     the library's path."""
-    BUILD.mkdir(exist_ok=True)
+    with _alone():
+        _build(force, verbose, jobs)
+    return LIB
+
+
+def _build(force: bool, verbose: bool, jobs: int | None) -> None:
     srcs = sorted(CSRC.glob("*.cu"))
     hdr_mtime = max((h.stat().st_mtime for h in _headers()), default=0.0)
     todo = []
@@ -118,8 +140,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
     if verbose:
         for name, log in sorted(logs.items()):
             print(f"== {name}\n{log}", file=sys.stderr)
-    build_binding(force)
-    return LIB
+    _build_binding(force)
 
 
 if __name__ == "__main__":

@@ -24,14 +24,14 @@ transform, for tensors of a subclass and where a gradient is wanted, they call t
 """
 from __future__ import annotations
 
-import importlib
+import importlib.util
 import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch.utils._device import DeviceContext
 
-from . import _lib
+from . import _build, _lib
 
 _bound = None
 
@@ -40,10 +40,14 @@ def _native():
     """The native binding, with the kernel library's entry points."""
     global _bound
     if _bound is None:
-        if not _lib.BINDING_PATH.exists() and _lib.autobuild():
-            from . import _build
+        path = _build.binding_path()
+        if not path.exists() and _lib.autobuild():
             _build.build()
-        module = importlib.import_module("._decoder", __package__)
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python -m triton_msl_b200._build`")
+        spec = importlib.util.spec_from_file_location(f"{__package__}._decoder", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
         lib = _lib.lib()
         module.bind(*(_lib.address(getattr(lib, f)) for f in (
             "b2_qk_norm_rope", "b2_kv_cache_write", "b2_kv_cache_read", "b2_kv_cache_attn", "b2_fa_packed",
