@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import triton_msl_b200 as b2
-from test_gpu_decoder_ops import U, attn_check, attn_ref, check, filled, gen, packed_check, packed_ref, randn
+from test_gpu_decoder_ops import U, attn_check, attn_ref, check, filled, gen, packed_check, packed_ref, pick, randn, row_values
 from triton_msl_b200 import _lib
 
 pytestmark = pytest.mark.gpu
@@ -101,6 +101,34 @@ def test_cache_attn_large_values_of_small_weight(dtype, D, group, N, large):
     check(got[:, :, 1::2], ref[:, :, 1::2], 2e-3 * top, dtype)
     # the outliers' own part: weight e^-40
     check(got[:, :, 0::2], ref[:, :, 0::2], 2e-3 * max(plain), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,group,Hq", [(128, 64, 4), (128, 64, 8), (128, 128, 16), (64, 64, 12)])
+def test_cache_attn_scores_of_large_terms(dtype, D, group, Hq):
+    # Queries of 30, nearly orthogonal to their sequence's key, beside a key of zeros whose value is 0 where the
+    # other's is 1: the result is the logistic function of a score whose terms reach hundreds. In log2 units the
+    # score is off by 2^-18 (the tensor core's sums of subnormal codes are low by that) + 2^-20 (its cut sums
+    # and the fp32 ones) of its parts; the function's slope is at most 1/4, the weights are rounded by 2^-11 each.
+    g = gen(68)
+    B = 200
+    cache, table = filled(g, [2] * B, 1, D, group, 16, garbage=False)
+    slots = table[:, 0].long()[:, None] * 16 + torch.arange(2, device="cuda")
+    k, v = torch.zeros(B, 2, 1, D, device="cuda"), torch.zeros(B, 2, 1, D, device="cuda")
+    k[:, 1, 0] = 2 * randn(g, B, D)
+    v[:, 1] = 1.0
+    b2.kv_cache_write(cache, k.view(2 * B, 1, D), v.view(2 * B, 1, D), slots.flatten())
+    kc, ks, _, _ = pick(cache, slots[:, 1])
+    held = row_values(kc, ks)[:, 0]  # [B, D]
+    q = 30 * randn(g, B, 1, Hq, D).double()
+    q = q - (q @ held[:, None, :, None]) / held.square().sum(-1)[:, None, None, None] * held[:, None, None]
+    q = q.to(dtype)
+    low = ks[:, 0, :, 1].double().repeat_interleave(group, -1)
+    size = max((q.double() @ part[:, None, :, None]).abs().max().item() for part in (low, held - low)) * D**-0.5 / math.log(2)
+    got = b2.kv_cache_attn(q, cache, table, torch.full((B,), 2, dtype=torch.int32, device="cuda"))
+    ref, _ = attn_ref(q, cache, table, [2] * B, D**-0.5)
+    assert 100 < size and 0.05 < ref.min() and ref.max() < 0.95
+    check(got, ref, 0.25 * math.log(2) * (2.0**-18 + 2.0**-20) * size + 2 * 2.0**-11 * 0.25, dtype)
 
 
 # -------------------------------------------------------------- packed prompts

@@ -6,13 +6,14 @@
 //   o_rd     = sum_j (p_rj sv_jg) cv_jd + sum_j p_rj lov_jg
 // so the codes themselves are what is multiplied, and scales and lowest values
 // touch one number per key and group, not one per channel. A 4-bit code c0 in the low
-// mantissa bits of an fp16 is the subnormal c0 * 2^-24, exactly, and a byte of two
-// codes is (c0 + 16 c1) * 2^-24. So a word of 8 codes becomes tensor-core operands,
-// for the c0 and for the bytes, by 4 instructions: q0 c0 + q1 c1 =
-// (q0 - q1/16) c0 + q1/16 (c0 + 16 c1), and the values' bytes give sums from which
-// the c0's are taken at the end (5 by taking c0 and 16 c1: 39.2 us where this
-// takes 37.7, 126 where 120). fp16 takes more for a more exact result (kBytes below).
-// The powers of two go into the last multiplication.
+// mantissa bits of an fp16 is the subnormal c0 * 2^-24, exactly, 16 c1 beside it is
+// 16 c1 * 2^-24, and a byte of two codes is (c0 + 16 c1) * 2^-24. So a word of 8 codes
+// becomes tensor-core operands by 5 instructions for keys, q0 c0 + q1/16 (16 c1), and by 4
+// for values, whose bytes give sums from which the c0's are taken at the end. q0 and
+// q1/16 are exact in fp16. (Bytes for the keys too want q0 - q1/16, which has to be
+// rounded: 1 to 1.5 % faster, 36.5 us where this takes 37.0, 116.4 where 118.2, but scores
+// of bf16 queries of 30 were off by up to 0.1.) For fp16 the values take more as well
+// (kBytes below). The powers of two go into the last multiplication.
 //
 // Tensor work is mma.sync m16n8k16 with the codes as the A operand, straight from
 // registers: S^T = K.Q^T (16 keys x 8 rows) and O^T = V^T.P^T (16 channels x 8
@@ -171,9 +172,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
   constexpr int NG = R::NG, N64 = D / 64, WPT = D / 32, ROWS = COLS * 4 * NT;
   // What bf16 results do not resolve and fp16 ones do (relative error of their output's
   // rounding 2.1e-4):
-  // - Keys' codes in bytes: the difference q0 - q1/16 is rounded to fp16 (2.8e-4 -> 3.9e-4
-  //   for 16 sequences of up to 4095 tokens). fp16 keeps q0 and q1/16, both exact, with c0
-  //   and 16 c1.
   // - Values' bytes as subnormals: their products' sums come out low by 2^-18 of their
   //   size. For fp16 the bytes lie 3 bits higher, where the largest are normal numbers
   //   (4 sequences of up to 42677 tokens: 3.9e-4 -> 2.4e-4).
@@ -181,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
   //   for each 16 keys a warp takes. For fp16 the codes' middle is taken from the sums
   //   after each tile, by the weights' own sum (64 key heads of 30000 tokens: 3.4e-4 ->
   //   2.9e-4, shift 7e-6 -> 5e-7 of values of 1).
-  // The three cost 32 sequences of up to 8192 tokens 40.4 us for bf16's 36.8, of up to
+  // The two cost 32 sequences of up to 8192 tokens 40.4 us for bf16's 36.8, of up to
   // 32768 130 for 117.
   constexpr bool kBytes = std::is_same<T, __nv_bfloat16>::value;
   constexpr float kUnit = kBytes ? 16777216.f : 2097152.f;  // of the sums of codes
@@ -357,9 +355,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             const int c0 = 8 * ii + 2 * s;
-            const float y0 = x[w][c0 + 1] * 0.0625f, y4 = x[w][c0 + 5] * 0.0625f;
-            qf[nt][ii * N64 + w][s][0] = kBytes ? half2_bits(x[w][c0] - y0, x[w][c0 + 4] - y4) : half2_bits(x[w][c0], x[w][c0 + 4]);
-            qf[nt][ii * N64 + w][s][1] = half2_bits(y0, y4);
+            qf[nt][ii * N64 + w][s][0] = half2_bits(x[w][c0], x[w][c0 + 4]);
+            qf[nt][ii * N64 + w][s][1] = half2_bits(x[w][c0 + 1] * 0.0625f, x[w][c0 + 5] * 0.0625f);
           }
       // to the lanes that hold the row's scores: columns 2t, 2t + 1
 #pragma unroll
@@ -420,8 +417,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
         for (int s = 0; s < 2; ++s) {
           const uint32_t x0 = s ? byte_pair(k0[w], 1) : k0[w], x1 = s ? byte_pair(k1[w], 1) : k1[w];
           const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu;
-          const uint32_t a2 = kBytes ? byte_pair(k0[w], s) : x0 & 0x00f000f0u;
-          const uint32_t a3 = kBytes ? byte_pair(k1[w], s) : x1 & 0x00f000f0u;
+          const uint32_t a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
             mma16816(acc[NG == 2 ? w % N64 : 0][nt], a0, a1, a2, a3, qf[nt][w][s][0], qf[nt][w][s][1]);
