@@ -131,6 +131,24 @@ def test_cache_attn_scores_of_large_terms(dtype, D, group, Hq):
     check(got, ref, 0.25 * math.log(2) * (2.0**-18 + 2.0**-20) * size + 2 * 2.0**-11 * 0.25, dtype)
 
 
+@pytest.mark.parametrize("D,group,Hq", [(64, 64, 16), (128, 64, 16), (128, 128, 96)])
+def test_cache_attn_sums_of_bf16_are_hardly_shifted(D, group, Hq):
+    # results far smaller than the values they are sums of. bf16's codes are subnormal operands: their sums, of
+    # the size of the values, come out low by 2^-18, and by 2^-25 for each 16 keys that a warp adds (some 16
+    # times here): together below 2^-17 of the largest value. Independent errors, of the weights (2^-11) and of
+    # the result (2^-9), average out over H * D channels, at 6 sigma.
+    g = gen(69 + D + Hq)
+    L, H = 30000, 16
+    cache, table = filled(g, [L], H, D, group, 64, extra=0)
+    b2.kv_cache_write(cache, randn(g, L, H, D) * 2, randn(g, L, H, D), slots_of(table, 0, torch.arange(L, device="cuda"), 64))
+    q = randn(g, 1, 1, Hq, D).bfloat16()
+    ref, top = attn_ref(q, cache, table, [L], D**-0.5)
+    got = b2.kv_cache_attn(q, cache, table, torch.tensor([L], dtype=torch.int32, device="cuda"))
+    shift = (got.double() - ref).mean().abs().item()
+    rms = ref.square().mean().sqrt().item()
+    assert shift <= 2.0**-17 * top.item() + 6 * (2.0**-11 + 2.0**-9) * rms / math.sqrt(H * D)
+
+
 # -------------------------------------------------------------- packed prompts
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("D", [64, 128])

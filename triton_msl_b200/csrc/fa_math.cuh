@@ -1,4 +1,4 @@
-// Softmax arithmetic of the tensor-core attention kernels: exponentials split between
+// Softmax arithmetic of the attention kernels: exponentials split between
 // the MUFU and the FMA pipe, packed fp32 pairs, three-input maxima.
 #pragma once
 #include <cuda_runtime.h>

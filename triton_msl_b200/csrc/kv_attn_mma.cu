@@ -44,10 +44,13 @@
 
 #include "b2_common.cuh"
 #include "decoder.cuh"
+#include "fa_math.cuh"
 #include "kv_attn.cuh"
 
 namespace b2 {
 namespace {
+
+using namespace fa;
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 2;
 constexpr int kSteps = 2;                    // of 16 keys a warp and tile
@@ -57,11 +60,6 @@ constexpr float kNoMax = -3e38f;
 // Bounds of log2(P * sv): where a row's m puts the largest, and where m is raised.
 constexpr float kPut = 8.f, kRaise = 15.5f;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -147,12 +145,6 @@ __device__ __forceinline__ unsigned count_units(const AttnArgs& a, int b, unsign
 // Bytes 0 and 2, or 1 and 3, of a word as the low bytes of two halves
 __device__ __forceinline__ uint32_t byte_pair(uint32_t x, int odd) {
   return odd ? __byte_perm(x, 0, 0x4341) : x & 0x00ff00ffu;
-}
-// 3-input maximum
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
-  return r;
 }
 
 // One row of the group: its token among the new ones and its query head.
@@ -467,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
     for (int u = 0; u < kSteps; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float y = max3(sv[u][h][0], sv[u][h][NG - 1], 8.9e-16f);  // NaN is left aside, here and below
+        const float y = fmax3(sv[u][h][0], sv[u][h][NG - 1], 8.9e-16f);  // NaN is left aside, here and below
         // exponent and first bits of the mantissa, as they lie in the word, behind 2^23
         log_sv[u][h] = fmaf(__uint_as_float(__byte_perm(__float_as_uint(y), 0x4b000000u, 0x7632)), 0.0078125f, -65663.f);
       }
@@ -478,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c2 = 0; c2 < COLS; ++c2)
-          over = max3(over, x[u][nt][c2] + log_sv[u][0], x[u][nt][2 + c2] + log_sv[u][1]);
+          over = fmax3(over, x[u][nt][c2] + log_sv[u][0], x[u][nt][2 + c2] + log_sv[u][1]);
     if (__any_sync(0xffffffffu, over > kRaise) || fresh) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -486,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
         for (int c2 = 0; c2 < COLS; ++c2) {
           float y = -INFINITY;
 #pragma unroll
-          for (int u = 0; u < kSteps; ++u) y = max3(y, x[u][nt][c2] + log_sv[u][0], x[u][nt][2 + c2] + log_sv[u][1]);
+          for (int u = 0; u < kSteps; ++u) y = fmax3(y, x[u][nt][c2] + log_sv[u][0], x[u][nt][2 + c2] + log_sv[u][1]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
           // the step; the first keys may set m below its start of 0. Whole numbers: what
