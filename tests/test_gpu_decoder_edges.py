@@ -149,6 +149,22 @@ def test_cache_attn_sums_of_bf16_are_hardly_shifted(D, group, Hq):
     assert shift <= 2.0**-17 * top.item() + 6 * (2.0**-11 + 2.0**-9) * rms / math.sqrt(H * D)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,group,Hq,N", [(64, 64, 4, 1), (128, 64, 4, 1), (128, 128, 8, 1), (128, 64, 4, 4), (64, 64, 24, 1)])
+def test_cache_attn_one_key_gives_its_value(dtype, D, group, Hq, N):
+    # The largest weight is a power of two, so its product with the value's scale is exact and not rounded by
+    # 2^-11. Left are the tensor core's sums of subnormal codes, low by 2^-18 of at most twice max|v|, and the
+    # result's one rounding.
+    g = gen(71)
+    lens = [N] * 40
+    cache, table = filled(g, lens, 1, D, group, 16)
+    q = randn(g, 40, N, Hq, D).to(dtype)
+    got = b2.kv_cache_attn(q, cache, table, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    _, _, vc, vs = pick(cache, table[:, 0].long() * 16)
+    want = row_values(vc, vs)  # [40, 1, D], token 0: all that the first new token sees
+    check(got[:, 0], want.expand(40, Hq, D), 2.0**-17 * want.abs().max(), dtype)
+
+
 # -------------------------------------------------------------- packed prompts
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("D", [64, 128])
