@@ -292,7 +292,8 @@ int b2_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, cons
  * A code c stands for c*scale + low, with low = min of the group rounded down to
  * bf16, scale = (max - low) * (1/15) rounded up to bf16 and, each operation in
  * fp32, c = rint((x - low) * (1/scale)).
- * A group that holds a NaN or an infinity reads back as NaN.
+ * A group that holds a NaN or an infinity, or whose range max - low passes fp32's,
+ * reads back as NaN.
  * Slot s is token s % page_size of page s / page_size.
  *
  * b2_kv_cache_write: quantises k[T, H, D] and v[T, H, D] into slots[T] (B2_I32 or

@@ -30,14 +30,15 @@
 // between CTAs is joined by kv_attn_join_kernel from partials in the workspace, in the
 // order of the keys.
 //
-// Bound: instructions (a third of them widen codes; ALU pipe 53 %, issue slots 57 %)
-// and, on long sequences, HBM. Measured, 32 query heads on 8, D = 128, groups of 64,
-// bf16: 32 sequences of up to 8192 tokens 36.8 us, 4.3 TB/s; of up to 32768 117 us, 5.3.
+// Bound: instructions, a third of which widen codes, and the waits between dependent ones
+// at 16 warps an SM (ALU pipe 56 %, issue slots 58 %), and, on long sequences, HBM.
+// Measured, 32 query heads on 8, D = 128, groups of 64, bf16: 32 sequences of up to 8192
+// tokens 37.2 us, 4.2 TB/s; of up to 32768 118.8 us, 5.3.
 //
 // Softmax: P = 2^(s - m), and P * sv is rounded to fp16 (the one rounding of weights,
-// 2^-11). So m follows the largest product P * sv of a row and not its largest score: it
-// starts 2^7 to 2^8 below the first, and is raised when one passes 2^15.5 (one vote a step). A
-// product of 2^-21 of the largest so far is not yet subnormal, and large values of small
+// 2^-11). So m follows the largest product P * sv of a row and not its largest score: the
+// first keys' lies at 2^7 to 2^8, and m is raised when one passes 2^15.5 (one vote a step).
+// A product of 2^-21 of the largest so far is not yet subnormal, and large values of small
 // weight leave the others their bits. Scores, sums, the lowest values' part and the
 // accumulators are fp32; P itself, at most 2^65.5, only meets those.
 #include <type_traits>
@@ -171,8 +172,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
   //   for each 16 keys a warp takes. For fp16 the codes' middle is taken from the sums
   //   after each tile, by the weights' own sum (64 key heads of 30000 tokens: 3.4e-4 ->
   //   2.9e-4, shift 7e-6 -> 5e-7 of values of 1).
-  // The two cost 32 sequences of up to 8192 tokens 40.4 us for bf16's 36.8, of up to
-  // 32768 130 for 117.
+  // The two cost 32 sequences of up to 8192 tokens 40.2 us for bf16's 37.2, of up to
+  // 32768 130 for 119.
   constexpr bool kBytes = std::is_same<T, __nv_bfloat16>::value;
   constexpr float kUnit = kBytes ? 16777216.f : 2097152.f;  // of the sums of codes
   // With a column to spare per row, the weights of a row's second group take it: one

@@ -15,7 +15,7 @@
 // rotation, 14 a value): vectors of 4 channels, 16 lanes a head of 128, leave
 // registers for 24 warps per SM. Measured on 16384 tokens, 32 + 8 heads of 128, norm,
 // half layout: bf16 56 us, 6.1 TB/s (4 heads a group 74; vectors of 8, 16 warps, and a
-// division per head in the norm 92); fp32 102 us, 6.7 TB/s.
+// division per head in the norm 92); fp32 102 to 111 us, 6.7 to 6.1 TB/s.
 #include <algorithm>
 #include <type_traits>
 

@@ -97,8 +97,10 @@ def rope_table(length: int, rot_dim: int, base: float = 10000.0, scaling: str = 
         slowest pair by ``factor`` and leaves the fastest
       * ``"by_parts"``: a pair that turns fewer than ``slow`` times in
         ``original_length`` positions is divided by ``factor``, one that turns more
-        than ``fast`` times is left, those between are blended; the table is
-        multiplied by 0.1*ln(factor) + 1 (YaRN, Peng et al. 2023)
+        than ``fast`` times is left, those between are blended linearly in the number
+        of turns; the table is multiplied by 0.1*ln(factor) + 1 (YaRN as published,
+        Peng et al. 2023). Models that blend by the channel's place instead, or leave
+        the table unscaled, bring a table of their own, which ``qk_norm_rope`` takes as well.
     Made once per model and kept; ``qk_norm_rope`` reads the rows of its positions.
     """
     what = "rope_table"
