@@ -165,6 +165,34 @@ def test_cache_attn_one_key_gives_its_value(dtype, D, group, Hq, N):
     check(got[:, 0], want.expand(40, Hq, D), 2.0**-17 * want.abs().max(), dtype)
 
 
+@pytest.mark.parametrize("D,group,Hq", [(128, 64, 4), (64, 64, 8), (128, 128, 24)])
+@pytest.mark.parametrize("size", [1e-25, 1e-12, 1e12, 1e30, 2e37])
+def test_cache_attn_values_of_every_size(D, group, Hq, size):
+    g = gen(72)
+    lens = [1, 300, 2000]
+    cache, table = filled(g, lens, 1, D, group, 16)
+    for b, n in enumerate(lens):
+        v = randn(g, n, 1, D).clamp(-4, 4) * size
+        v[n // 3:n // 2] = 0  # a part without any
+        b2.kv_cache_write(cache, randn(g, n, 1, D) * 2, v, slots_of(table, b, torch.arange(n, device="cuda"), 16))
+    attn_check(randn(g, 3, 1, Hq, D).bfloat16(), cache, table, lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value", [0.0, 1.0, -6e4])
+def test_cache_attn_constant_values(dtype, value):
+    # every group's scale is 0: the result is the value itself, however the scores are spread
+    g = gen(73)
+    lens, D = [1, 50, 20000], 128
+    cache, table = filled(g, lens, 1, D, 64, 64)
+    for b, n in enumerate(lens):
+        k = randn(g, n, 1, D) * torch.linspace(0.1, 4, n, device="cuda")[:, None, None]
+        b2.kv_cache_write(cache, k, torch.full((n, 1, D), value, device="cuda").bfloat16().float(),
+                          slots_of(table, b, torch.arange(n, device="cuda"), 64))
+    attn_check(randn(g, 3, 2, 4, D).to(dtype)[:, 1:], cache, table, lens)
+    attn_check(3 * randn(g, 3, 2, 8, D).to(dtype)[:, 1:], cache, table, lens)
+
+
 # -------------------------------------------------------------- packed prompts
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("D", [64, 128])

@@ -40,7 +40,7 @@
 // first keys' lies at 2^7 to 2^8, and m is raised when one passes 2^15.5 (one vote a step).
 // A product of 2^-21 of the largest so far is not yet subnormal, and large values of small
 // weight leave the others their bits. Scores, sums, the lowest values' part and the
-// accumulators are fp32; P itself, at most 2^65.5, only meets those.
+// accumulators are fp32; P itself, at most 2^85.5, only meets those.
 #include <type_traits>
 
 #include "b2_common.cuh"
@@ -455,12 +455,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D, NT>) kv_attn_kernel(co
         }
     }
     // raise the references where needed
-    float log_sv[kSteps][2];  // of the larger scale, at least -50: 0.1 too low at most
+    float log_sv[kSteps][2];  // of the larger scale, at least -70: 0.1 too low at most
 #pragma unroll
     for (int u = 0; u < kSteps; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float y = fmax3(sv[u][h][0], sv[u][h][NG - 1], 8.9e-16f);  // NaN is left aside, here and below
+        const float y = fmax3(sv[u][h][0], sv[u][h][NG - 1], 8.5e-22f);  // NaN is left aside, here and below
         // exponent and first bits of the mantissa, as they lie in the word, behind 2^23
         log_sv[u][h] = fmaf(__uint_as_float(__byte_perm(__float_as_uint(y), 0x4b000000u, 0x7632)), 0.0078125f, -65663.f);
       }
