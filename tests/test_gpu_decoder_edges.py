@@ -261,6 +261,23 @@ def test_packed_offsets_that_descend(dtype, cu, clamped):
     check(got, ref, 1e-4 if dtype == torch.float32 else (U[dtype] + 3e-4) * top, dtype)
 
 
+def test_packed_prompts_of_millions_of_tokens():
+    # seconds of units whose last key block is full, between others where it is not: no wait that spans them
+    # may take that for a stalled pipeline
+    g = gen(74)
+    lens, H, D = [2097152, 1200005], 4, 64
+    T = sum(lens)
+    q, k, v = (torch.empty(T, H, D, device="cuda", dtype=torch.bfloat16).normal_(generator=g) for _ in range(3))
+    cu = [0, lens[0], T]
+    got = b2.flash_attn_packed(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"))
+    assert b2.last_kernel() == "fa_packed_sm100" and b2.device_status(0) == 0
+    for b, i in ((0, 5), (0, lens[0] // 2 + 3), (0, lens[0] - 1), (1, 0), (1, 700001), (1, lens[1] - 1)):
+        keys = slice(cu[b], cu[b] + i + 1)
+        p = torch.softmax(torch.einsum("hd,jhd->hj", q[cu[b] + i].double(), k[keys].double()) * D**-0.5, 1)
+        ref = torch.einsum("hj,jhd->hd", p, v[keys].double())
+        check(got[cu[b] + i], ref, (U[torch.bfloat16] + 3e-4) * v[keys].abs().max().double().item(), torch.bfloat16)
+
+
 # ------------------------------------------------------------------ how they are called
 def test_the_binding_refuses_tensors_without_storage():
     # what a transform wraps has no storage: an exception, and not the end of the process

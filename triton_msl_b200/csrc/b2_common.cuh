@@ -32,7 +32,8 @@ enum : uint32_t {
 };
 
 // Upper bound on any single spin inside a kernel. Every legitimate wait in
-// these kernels is microseconds; one second means the pipeline is wedged.
+// these kernels is microseconds (one that may span more work watches its progress);
+// one second means the pipeline is wedged.
 constexpr unsigned long long kWaitLimitNs = 1000ull * 1000ull * 1000ull;
 
 inline int dtype_size(int dt) {

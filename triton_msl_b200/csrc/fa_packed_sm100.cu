@@ -171,6 +171,7 @@ struct __align__(8) Barriers {
   uint64_t done;
   uint32_t tmem_base;
   int abort_flag;
+  uint32_t blocks;  // that warp 0 has asked for
 };
 
 template <int D>
@@ -221,6 +222,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &bars->abort_flag;
+  volatile uint32_t* blocks = &bars->blocks;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
@@ -238,6 +240,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
     mbar_init(&bars->done, 1);
     bars->abort_flag = 0;
+    bars->blocks = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
@@ -344,6 +347,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int at = 0; at < C::kAtoms; ++at)
             tma_load_3d(sV + s * C::kTileBytes + at * C::kAtomTileBytes, &tmV, vbar, at * 64, u.kvh,
                         u.e.k0 + j * kBN);
+          *blocks = g + 1;
         }
       }
       // Bounded drain of copies still in flight into this CTA's shared memory.
@@ -476,6 +480,27 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsProducer));
     uint32_t g = 0;
     uint32_t tails = 0;  // bit s: phase of vt_full[s]
+    // Units without such rows are passed over, so a wait can span many of them: seconds
+    // in a batch of prompts of a million tokens. It ends when no block is asked for any more.
+    auto wait_tail = [&](uint64_t* bar, uint32_t parity) {
+      const uint32_t at = smem_addr(bar);
+      uint32_t seen = *blocks;
+      unsigned long long t0 = globaltimer();
+      for (uint32_t it = 1; !mbar_test(at, parity); ++it) {
+        if ((it & 63u) != 0) continue;
+        if (*abort_flag) return false;
+        const uint32_t now = *blocks;
+        if (now != seen) {
+          seen = now;
+          t0 = globaltimer();
+        } else if (globaltimer() - t0 > kWaitLimitNs) {
+          *abort_flag = 1;
+          atomicOr(&g_packed_status, DEV_TIMEOUT_TMA);
+          return false;
+        }
+      }
+      return true;
+    };
     Unit next = fetch(0);
     for (uint32_t ui = 0; next.valid; ++ui) {
       const Unit u = next;
@@ -484,9 +509,7 @@ fa_packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       g += n;
       if (n == 0 || !has_tail(u.e, n)) continue;
       const int s = (g - 1) & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars->vt_full[s], (tails >> s) & 1u, abort_flag, &g_packed_status,
-                                             DEV_TIMEOUT_TMA)))
-        break;
+      if (!__all_sync(0xffffffffu, wait_tail(&bars->vt_full[s], (tails >> s) & 1u))) break;
       tails ^= 1u << s;
       const int first = u.e.Lk - (n - 1) * kBN;  // 1 .. 127: rows from here on are not the sequence's
       uint8_t* v = sV + s * C::kTileBytes;
